@@ -431,6 +431,93 @@ SA_API int sa_paged_append_kv(const void *k_new, const void *v_new, void *k_page
                               int64_t num_pages, int layout, int64_t new_stride_b, int64_t new_stride_h,
                               int dtype, int *status, sa_stream_t stream);
 
+/* ---- 8-bit KV caches -------------------------------------------------------------------------
+ * A cache row - one token of one KV head, head_dim values of K or V - is held as head_dim codes of
+ * 8 bits and one power-of-two scale 2^(e - 127) stored as the byte e (255 = NaN):
+ *   e     the smallest exponent with max|x| <= top * 2^(e - 127), top = 448 (e4m3) or 127 (int8),
+ *         at least 27 (smaller rows lose precision towards zero)
+ *   code  x / 2^(e - 127), exact, then rounded to the code's type (halves to even)
+ * A row that holds an infinity or a NaN gets e = 255 and codes 0: it reads back as NaN and makes
+ * the outputs of its KV head NaN.  The power of two makes the codes independent of the arithmetic
+ * that computed them, the read-back into 16-bit types exact and a second quantisation idempotent.
+ * Scales lie head-major whatever the codes' layout is, the K and the V byte of a token side by
+ * side.  No counterpart in the reference. */
+enum sa_kv_code { SA_KV_E4M3 = 1, SA_KV_INT8 = 2 };
+
+typedef struct sa_quant_cache {
+    void *key;                  /* codes of the K rows                                              */
+    void *value;                /* codes of the V rows, same shape and strides                      */
+    void *scales;               /* uint8 pairs: [batch, kv_heads, capacity, 2] (contiguous cache) or
+                                   [num_pages, kv_heads, page_size, 2] (paged, no gaps)             */
+    int code;                   /* sa_kv_code                                                       */
+    int batch, kv_heads, head_dim;
+    /* contiguous cache (page_table == NULL): strides of the codes in codes, of the scales in pairs */
+    int64_t capacity;
+    int64_t stride_b, stride_n, stride_h;
+    int64_t scale_stride_b, scale_stride_h;
+    /* paged cache: pages [num_pages, page_size, kv_heads, D] (NHD) or [num_pages, kv_heads, page_size, D] (HND) */
+    const void *page_table;     /* [batch, max_pages]                                               */
+    int table_dtype;
+    int page_size, max_pages;
+    int64_t num_pages;
+    int layout;
+} sa_quant_cache_t;
+
+/*
+ * Quantise `tokens` new rows per batch row and KV head into the cache at positions
+ * [position, position + count), after rotating K (x * cos + rotate_half(x) * sin, computed in fp32,
+ * not rounded before the quantisation) where cos / sin are given.
+ *   k_new, v_new   [batch, tokens, kv_heads, D], strides in elements (D contiguous), dtype `dtype`
+ *   positions      device int32/int64, one entry or one per row: token index of the first new row
+ *   counts         optional device array [batch]: new tokens of each row, clipped to [0, tokens]
+ *                  (the rest of its rows is padding and not read); NULL = tokens
+ *   lens_out       optional device array [batch] (type of positions): position + count; may be the
+ *                  per-row `positions` itself
+ *   cos, sin       optional [batch or 1, tokens, D], dtype `dtype` (rope_stride_b = 0: shared)
+ *   q_in / q_out   optional [batch, tokens, q_heads, D]: the query rotated (fp32, rounded once) or,
+ *                  without cos / sin, copied; q_out must not alias q_in
+ *   status         optional device int32.  A row whose tokens do not fit the cache is left out as a
+ *                  whole (SA_DEV_BAD_POSITION), a token whose page id is out of range is skipped
+ *                  (SA_DEV_BAD_PAGE); in both cases the row's entry of lens_out is not written.
+ * One launch, or two when lens_out is given and a row's tokens need more than one CTA.
+ */
+SA_API int sa_quantize_kv(const sa_quant_cache_t *cache, const void *k_new, const void *v_new, int64_t tokens,
+                          int64_t new_stride_b, int64_t new_stride_t, int64_t new_stride_h,
+                          const void *positions, int pos_dtype, int num_positions,
+                          const void *counts, int counts_dtype, void *lens_out,
+                          const void *cos, const void *sin, int64_t rope_stride_b, int64_t rope_stride_t,
+                          const void *q_in, void *q_out, int q_heads,
+                          int64_t q_in_stride_b, int64_t q_in_stride_t, int64_t q_in_stride_h,
+                          int64_t q_out_stride_b, int64_t q_out_stride_t, int64_t q_out_stride_h,
+                          int dtype, int *status, sa_stream_t stream);
+
+/*
+ * Read tokens [start, start + count) of every row back as K and V of `dtype`:
+ * out [batch, tokens, kv_heads, D] (strides in elements, D contiguous); rows behind a row's count
+ * are left as they were.  starts (NULL = 0) and counts (NULL = tokens) are optional device arrays
+ * [batch]; a token outside the cache or with a bad page id is left out and reported as above.
+ */
+SA_API int sa_dequantize_kv(const sa_quant_cache_t *cache, void *k_out, void *v_out, int64_t tokens,
+                            int64_t out_stride_b, int64_t out_stride_t, int64_t out_stride_h,
+                            const void *starts, int starts_dtype, const void *counts, int counts_dtype,
+                            int dtype, int *status, sa_stream_t stream);
+
+/*
+ * Exact decode over an 8-bit cache: softmax(q K'^T / sqrt(D)) V' with K', V' the values the codes
+ * stand for; everything else as sa_exact_decode (contiguous cache; seq_lens NULL = capacity) and
+ * sa_paged_decode (paged cache; seq_lens required, trace optional).  The plan form is run with
+ * sa_plan_run and takes sa_plan_set_rows and sa_plan_set_wait_limit_ns.  Tokens of a bad page are
+ * left out of the softmax and reported (SA_DEV_BAD_PAGE).
+ */
+SA_API int sa_quant_decode(const void *q, const sa_quant_cache_t *cache, void *out,
+                           void *workspace, size_t workspace_bytes, const void *seq_lens, int lens_dtype,
+                           int32_t *trace, int q_heads, int64_t q_stride_b, int64_t q_stride_h,
+                           int dtype, int out_mode, int num_ctas, int kernel_choice, sa_stream_t stream);
+SA_API sa_plan_t *sa_quant_plan_create(const void *q, const sa_quant_cache_t *cache, void *out,
+                                       void *workspace, size_t workspace_bytes, const void *seq_lens, int lens_dtype,
+                                       int32_t *trace, int q_heads, int64_t q_stride_b, int64_t q_stride_h,
+                                       int dtype, int out_mode, int num_ctas, int kernel_choice);
+
 /* ---- Output projection: the step after each decode call ----------------------------------
  * out[b, n] = sum_k x[b, k] * weight[n, k] (+ bias[n]) for the few rows of a decode step, fp32
  * accumulation, result in the input dtype (bf16/fp16).  Replaces qwen_o_proj_triton_forward

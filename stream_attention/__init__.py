@@ -31,6 +31,8 @@ _ALIASES = {
     "seed_autotune": "streamattn_b200.seed_autotune",
     "bucket_policy": "streamattn_b200.bucket_policy",
     "kv_update": "streamattn_b200.kv_update",
+    "quant_cache": "streamattn_b200.quant_cache",
+    "quant_kv": "streamattn_b200.quant_kv",
     "context_parallel": "streamattn_b200.context_parallel",
     # the reference's sm_90 backend package: the bound exact plan lives there
     "backends.sm90": "streamattn_b200.exact",

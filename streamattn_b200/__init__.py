@@ -69,6 +69,17 @@ from .bucket_policy import (
 )
 from .o_proj import OProjPlan, qwen_o_proj_forward
 from .kv_update import AppendKVPlan, PagedKVWriter, PagePool, append_kv, paged_append_kv
+from .quant_cache import QuantKVCache, QuantPagedKVCache
+from .quant_kv import (
+    QUANT_EXACT_NATIVE_BACKEND,
+    QUANT_EXACT_SM100_BACKEND,
+    DequantizeKVPlan,
+    QuantDecodePlan,
+    QuantizeKVPlan,
+    dequantize_kv,
+    quantize_kv,
+    stream_attn_quant_decode,
+)
 from .seed_selectors import (
     DynamicSeedDecodePlan,
     SeedBlockSelection,

@@ -7,11 +7,13 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <vector>
 
 #include "sa_append.cuh"
+#include "sa_quant.cuh"
 #include "sa_stream.cuh"
 
 namespace sa {
@@ -148,6 +150,7 @@ bool build_stream_geometry(const Problem &p, int64_t max_vlen, StreamGeometry *g
 {
     *why = "";
     if (p.dtype != SA_DTYPE_BF16 && p.dtype != SA_DTYPE_F16) { *why = "dtype is not bf16/fp16"; return false; }
+    if (p.quant.code != kCodeNone) { *why = "8-bit cache"; return false; }
     if (p.head_dim != 64 && p.head_dim != 128) { *why = "head_dim is not 64 or 128"; return false; }
     geo->kv_split = stream_kv_split(p.q_heads / p.kv_heads);
     if (geo->kv_split == 0) { *why = "query heads per KV head cannot be split into groups of at most 16"; return false; }
@@ -463,6 +466,109 @@ int fill_seed_device(sa_plan *plan, const void *q, const void *k, const void *v,
     p.seq.blocks_vlen = static_cast<int64_t>(blocks_per_pair) * block_size - clip;
     p.num_ctas = num_ctas;
     return finish_plan(plan, workspace, workspace_bytes, p.seq.blocks_vlen, kernel_choice);
+}
+
+// An 8-bit cache as the caller describes it: checks, and the descriptor of the row kernels.
+int fill_quant_cache(QuantCache *c, const sa_quant_cache_t *d)
+{
+    if (!d) return fail(SA_ERR_INVALID, "null cache descriptor");
+    if (!d->key || !d->value || !d->scales) return fail(SA_ERR_INVALID, "null tensor pointer");
+    if (d->code != SA_KV_E4M3 && d->code != SA_KV_INT8) return fail(SA_ERR_INVALID, "unknown cache code type");
+    if (d->batch <= 0 || d->kv_heads <= 0) return fail(SA_ERR_INVALID, "batch/heads must be positive");
+    if (d->head_dim <= 0 || d->head_dim > 256) return fail(SA_ERR_INVALID, "head_dim must be in [1, 256]");
+    if (reinterpret_cast<uintptr_t>(d->scales) % 2) return fail(SA_ERR_INVALID, "scales must be 2-byte aligned");
+    std::memset(c, 0, sizeof(*c));
+    c->key = static_cast<uint8_t *>(d->key);
+    c->value = static_cast<uint8_t *>(d->value);
+    c->scales = static_cast<uint8_t *>(d->scales);
+    c->kv_heads = d->kv_heads;
+    c->head_dim = d->head_dim;
+    c->page_shift = -1;
+    int64_t capacity;
+    if (d->page_table == nullptr) {
+        if (d->capacity <= 0) return fail(SA_ERR_INVALID, "the cache's capacity must be positive");
+        if (d->stride_n <= 0 || d->stride_h < 0 || d->stride_b < 0 || d->scale_stride_b < 0 || d->scale_stride_h < 0)
+            return fail(SA_ERR_INVALID, "non-positive KV stride");
+        capacity = d->capacity;
+        c->so = d->stride_b; c->sn = d->stride_n; c->sh = d->stride_h;
+        c->scale_so = d->scale_stride_b; c->scale_sh = d->scale_stride_h;
+    } else {
+        if (d->page_size <= 0 || d->max_pages <= 0 || d->num_pages <= 0)
+            return fail(SA_ERR_INVALID, "paged cache dimensions must be positive");
+        if (d->layout != SA_LAYOUT_NHD && d->layout != SA_LAYOUT_HND)
+            return fail(SA_ERR_INVALID, "paged KV layout must be NHD or HND");
+        if (d->table_dtype != SA_INDEX_I32 && d->table_dtype != SA_INDEX_I64)
+            return fail(SA_ERR_INVALID, "page_table must be int32 or int64");
+        capacity = static_cast<int64_t>(d->max_pages) * d->page_size;
+        const int64_t rows = static_cast<int64_t>(d->page_size) * d->kv_heads;
+        c->so = rows * d->head_dim;
+        c->sn = d->layout == SA_LAYOUT_NHD ? static_cast<int64_t>(d->kv_heads) * d->head_dim : d->head_dim;
+        c->sh = d->layout == SA_LAYOUT_NHD ? d->head_dim : static_cast<int64_t>(d->page_size) * d->head_dim;
+        c->scale_so = rows;
+        c->scale_sh = d->page_size;
+        c->page_table = d->page_table;
+        c->table_i64 = d->table_dtype == SA_INDEX_I64;
+        c->max_pages = d->max_pages;
+        c->page_size = d->page_size;
+        c->num_pages = d->num_pages;
+        if (is_pow2(d->page_size))
+            for (c->page_shift = 0; (1 << c->page_shift) < d->page_size;) ++c->page_shift;
+    }
+    if (capacity >= (1ll << 31)) return fail(SA_ERR_UNSUPPORTED, "rows of 2^31 tokens or more");
+    c->capacity = static_cast<int>(capacity);
+    return SA_OK;
+}
+
+// Exact decode over an 8-bit cache.
+int fill_quant(sa_plan *plan, const void *q, const sa_quant_cache_t *cache, void *out, void *workspace,
+               size_t workspace_bytes, const void *seq_lens, int lens_dtype, int32_t *trace, int q_heads, int64_t q_sb,
+               int64_t q_sh, int dtype, int out_mode, int num_ctas, int kernel_choice)
+{
+    QuantCache c;
+    int rc = fill_quant_cache(&c, cache);
+    if (rc) return rc;
+    rc = check_common(q, c.key, c.value, out, workspace, cache->batch, q_heads, c.kv_heads, c.head_dim, dtype, out_mode,
+                      num_ctas, kernel_choice);
+    if (rc) return rc;
+    if (lens_dtype != SA_INDEX_I32 && lens_dtype != SA_INDEX_I64) return fail(SA_ERR_INVALID, "unknown lens_dtype");
+    const bool paged = c.page_table != nullptr;
+    if (paged && !seq_lens) return fail(SA_ERR_INVALID, "page_table and seq_lens are required");
+    std::memset(plan, 0, sizeof(*plan));
+    Problem &p = plan->problem;
+    p.q = q; p.k = c.key; p.v = c.value; p.out = out;
+    p.dtype = dtype; p.out_mode = out_mode;
+    p.batch = cache->batch; p.q_heads = q_heads; p.kv_heads = c.kv_heads; p.head_dim = c.head_dim;
+    p.q_sb = q_sb; p.q_sh = q_sh;
+    p.seq.mode = paged ? kPaged : kContig;
+    p.seq.num_rows = -1;
+    p.seq.seq_lens = seq_lens;
+    p.seq.lens_i64 = lens_dtype == SA_INDEX_I64;
+    if (paged) {
+        p.seq.page_table = c.page_table;
+        p.seq.table_i64 = c.table_i64;
+        p.seq.max_pages = c.max_pages;
+        p.seq.page_size = c.page_size;
+        p.seq.num_pages = c.num_pages;
+        p.seq.pg_sp = c.so; p.seq.pg_st = c.sn; p.seq.pg_sh = c.sh;
+        p.trace = trace;
+    } else {
+        p.seq.kv_sb = c.so; p.seq.kv_sn = c.sn; p.seq.kv_sh = c.sh;
+        p.seq.kv_len = c.capacity;
+    }
+    p.quant.code = cache->code;
+    p.quant.scales = c.scales;
+    p.quant.so = c.scale_so; p.quant.sh = c.scale_sh;
+    p.num_ctas = num_ctas;
+    return finish_plan(plan, workspace, workspace_bytes, c.capacity, kernel_choice);
+}
+
+// Whether rows of `stride`-spaced elements of `size` bytes can be moved in 16-byte pieces.
+bool wide(const void *p, std::initializer_list<int64_t> strides, int size, int align)
+{
+    if (reinterpret_cast<uintptr_t>(p) % align) return false;
+    for (int64_t s : strides)
+        if (s * size % align) return false;
+    return true;
 }
 
 }  // namespace
@@ -1089,6 +1195,129 @@ int sa_o_proj(const void *x, const void *weight, const void *bias, void *out, in
     const cudaError_t err = launch_o_proj(x, weight, bias, out, batch, in_features, out_features, x_stride_b, dtype,
                                           prefetch_weights != 0, static_cast<cudaStream_t>(stream));
     if (err != cudaSuccess) return fail_cuda(err, "sa_o_proj");
+    return SA_OK;
+}
+
+int sa_quant_decode(const void *q, const sa_quant_cache_t *cache, void *out, void *workspace, size_t workspace_bytes,
+                    const void *seq_lens, int lens_dtype, int32_t *trace, int q_heads, int64_t q_stride_b,
+                    int64_t q_stride_h, int dtype, int out_mode, int num_ctas, int kernel_choice, sa_stream_t stream)
+{
+    sa_plan plan;
+    const int rc = fill_quant(&plan, q, cache, out, workspace, workspace_bytes, seq_lens, lens_dtype, trace, q_heads,
+                              q_stride_b, q_stride_h, dtype, out_mode, num_ctas, kernel_choice);
+    if (rc) return rc;
+    return run_plan(&plan, static_cast<cudaStream_t>(stream));
+}
+
+sa_plan_t *sa_quant_plan_create(const void *q, const sa_quant_cache_t *cache, void *out, void *workspace,
+                                size_t workspace_bytes, const void *seq_lens, int lens_dtype, int32_t *trace,
+                                int q_heads, int64_t q_stride_b, int64_t q_stride_h, int dtype, int out_mode,
+                                int num_ctas, int kernel_choice)
+{
+    sa_plan *plan = new (std::nothrow) sa_plan;
+    if (!plan) return nullptr;
+    if (fill_quant(plan, q, cache, out, workspace, workspace_bytes, seq_lens, lens_dtype, trace, q_heads, q_stride_b,
+                   q_stride_h, dtype, out_mode, num_ctas, kernel_choice)) {
+        delete plan;
+        return nullptr;
+    }
+    return plan;
+}
+
+int sa_quantize_kv(const sa_quant_cache_t *cache, const void *k_new, const void *v_new, int64_t tokens,
+                   int64_t new_stride_b, int64_t new_stride_t, int64_t new_stride_h, const void *positions,
+                   int pos_dtype, int num_positions, const void *counts, int counts_dtype, void *lens_out,
+                   const void *cos, const void *sin, int64_t rope_stride_b, int64_t rope_stride_t, const void *q_in,
+                   void *q_out, int q_heads, int64_t q_in_stride_b, int64_t q_in_stride_t, int64_t q_in_stride_h,
+                   int64_t q_out_stride_b, int64_t q_out_stride_t, int64_t q_out_stride_h, int dtype, int *status,
+                   sa_stream_t stream)
+{
+    QuantizeParams a;
+    std::memset(&a, 0, sizeof(a));
+    const int rc = fill_quant_cache(&a.cache, cache);
+    if (rc) return rc;
+    if (!k_new || !v_new || !positions) return fail(SA_ERR_INVALID, "null tensor pointer");
+    if (tokens <= 0) return fail(SA_ERR_INVALID, "tokens must be positive");
+    if (dtype < SA_DTYPE_BF16 || dtype > SA_DTYPE_F32) return fail(SA_ERR_INVALID, "unknown dtype");
+    if (pos_dtype != SA_INDEX_I32 && pos_dtype != SA_INDEX_I64)
+        return fail(SA_ERR_INVALID, "positions must be int32 or int64");
+    if (counts && counts_dtype != SA_INDEX_I32 && counts_dtype != SA_INDEX_I64)
+        return fail(SA_ERR_INVALID, "counts must be int32 or int64");
+    if (num_positions != 1 && num_positions != cache->batch)
+        return fail(SA_ERR_INVALID, "positions must hold one entry or one per batch row");
+    if (lens_out == positions && num_positions == 1 && cache->batch > 1)
+        return fail(SA_ERR_INVALID, "lens_out may alias positions only when there is one position per row");
+    if (lens_out && lens_out == counts) return fail(SA_ERR_INVALID, "lens_out must not alias counts");
+    if ((cos == nullptr) != (sin == nullptr)) return fail(SA_ERR_INVALID, "cos and sin must be given together");
+    if (cos && a.cache.head_dim % 2) return fail(SA_ERR_INVALID, "rotary embedding needs an even head_dim");
+    if ((q_in == nullptr) != (q_out == nullptr)) return fail(SA_ERR_INVALID, "q_in and q_out must be given together");
+    if (q_in && (q_heads <= 0 || q_heads % a.cache.kv_heads))
+        return fail(SA_ERR_INVALID, "query heads must be a positive multiple of KV heads");
+    if (q_in && q_in == q_out) return fail(SA_ERR_INVALID, "q_out must not alias q_in");
+    if (cache->batch > 65535) return fail(SA_ERR_UNSUPPORTED, "batch larger than 65535");
+    const int64_t heads = q_in ? std::max(q_heads, a.cache.kv_heads) : a.cache.kv_heads;
+    if (tokens > (1ll << 30) / heads) return fail(SA_ERR_UNSUPPORTED, "more than 2^30 new rows per batch row");
+    a.k_new = k_new; a.v_new = v_new;
+    a.new_sb = new_stride_b; a.new_st = new_stride_t; a.new_sh = new_stride_h;
+    a.tokens = static_cast<int>(tokens);
+    a.batch = cache->batch;
+    a.positions = positions;
+    a.pos_i64 = pos_dtype == SA_INDEX_I64;
+    a.pos_shared = num_positions == 1;
+    a.counts = counts;
+    a.counts_i64 = counts_dtype == SA_INDEX_I64;
+    a.lens_out = lens_out;
+    a.cos = cos; a.sin = sin; a.rope_sb = rope_stride_b; a.rope_st = rope_stride_t;
+    a.q_in = q_in; a.q_out = q_out; a.q_heads = q_heads;
+    a.qi_sb = q_in_stride_b; a.qi_st = q_in_stride_t; a.qi_sh = q_in_stride_h;
+    a.qo_sb = q_out_stride_b; a.qo_st = q_out_stride_t; a.qo_sh = q_out_stride_h;
+    a.status = status;
+    a.heads_fastest = new_stride_h <= new_stride_t;
+    const int size = dtype == SA_DTYPE_F32 ? 4 : 2;
+    const QuantCache &c = a.cache;
+    bool vector = c.head_dim % 8 == 0 && wide(k_new, {new_stride_b, new_stride_t, new_stride_h}, size, 16) &&
+                  wide(v_new, {}, size, 16) && wide(c.key, {c.so, c.sn, c.sh}, 1, 8) && wide(c.value, {}, 1, 8);
+    if (cos) vector = vector && c.head_dim % 16 == 0 && wide(cos, {rope_stride_b, rope_stride_t}, size, 16) && wide(sin, {}, size, 16);
+    if (q_in)
+        vector = vector && wide(q_in, {q_in_stride_b, q_in_stride_t, q_in_stride_h}, size, 16) &&
+                 wide(q_out, {q_out_stride_b, q_out_stride_t, q_out_stride_h}, size, 16);
+    const cudaError_t err = launch_quantize(a, cache->code, dtype, vector, static_cast<cudaStream_t>(stream));
+    if (err != cudaSuccess) return fail_cuda(err, "kernel launch failed");
+    return SA_OK;
+}
+
+int sa_dequantize_kv(const sa_quant_cache_t *cache, void *k_out, void *v_out, int64_t tokens, int64_t out_stride_b,
+                     int64_t out_stride_t, int64_t out_stride_h, const void *starts, int starts_dtype,
+                     const void *counts, int counts_dtype, int dtype, int *status, sa_stream_t stream)
+{
+    DequantizeParams a;
+    std::memset(&a, 0, sizeof(a));
+    const int rc = fill_quant_cache(&a.cache, cache);
+    if (rc) return rc;
+    if (!k_out || !v_out) return fail(SA_ERR_INVALID, "null tensor pointer");
+    if (tokens <= 0) return fail(SA_ERR_INVALID, "tokens must be positive");
+    if (dtype < SA_DTYPE_BF16 || dtype > SA_DTYPE_F32) return fail(SA_ERR_INVALID, "unknown dtype");
+    if ((starts && starts_dtype != SA_INDEX_I32 && starts_dtype != SA_INDEX_I64) ||
+        (counts && counts_dtype != SA_INDEX_I32 && counts_dtype != SA_INDEX_I64))
+        return fail(SA_ERR_INVALID, "starts and counts must be int32 or int64");
+    if (cache->batch > 65535) return fail(SA_ERR_UNSUPPORTED, "batch larger than 65535");
+    if (tokens > (1ll << 30) / a.cache.kv_heads) return fail(SA_ERR_UNSUPPORTED, "more than 2^30 rows per batch row");
+    a.k_out = k_out; a.v_out = v_out;
+    a.out_sb = out_stride_b; a.out_st = out_stride_t; a.out_sh = out_stride_h;
+    a.tokens = static_cast<int>(tokens);
+    a.batch = cache->batch;
+    a.starts = starts;
+    a.starts_i64 = starts_dtype == SA_INDEX_I64;
+    a.counts = counts;
+    a.counts_i64 = counts_dtype == SA_INDEX_I64;
+    a.status = status;
+    a.heads_fastest = a.cache.sh <= a.cache.sn;
+    const int size = dtype == SA_DTYPE_F32 ? 4 : 2;
+    const QuantCache &c = a.cache;
+    const bool vector = c.head_dim % 8 == 0 && wide(k_out, {out_stride_b, out_stride_t, out_stride_h}, size, 16) &&
+                        wide(v_out, {}, size, 16) && wide(c.key, {c.so, c.sn, c.sh}, 1, 8) && wide(c.value, {}, 1, 8);
+    const cudaError_t err = launch_dequantize(a, cache->code, dtype, vector, static_cast<cudaStream_t>(stream));
+    if (err != cudaSuccess) return fail_cuda(err, "kernel launch failed");
     return SA_OK;
 }
 

@@ -90,6 +90,16 @@ struct Workspace {
     size_t partial_floats;
 };
 
+enum KvCode : int { kCodeNone = 0, kCodeE4M3 = SA_KV_E4M3, kCodeInt8 = SA_KV_INT8 };
+
+// Scale bytes of an 8-bit cache: the (K, V) pair of a token is pair outer * so + head * sh + token,
+// `outer` and `token` being row and position, or page and slot.
+struct QuantScales {
+    int code;              // KvCode; kCodeNone: the cache holds elements of the query's type
+    const uint8_t *scales;
+    int64_t so, sh;
+};
+
 // Everything a launch needs; filled by the entry points in sa_api.cu.
 struct Problem {
     const void *q;
@@ -101,6 +111,7 @@ struct Problem {
     int batch, q_heads, kv_heads, head_dim;
     int64_t q_sb, q_sh;
     SeqDesc seq;
+    QuantScales quant;
     Workspace ws;
     int32_t *trace;
     int num_ctas;  // requested (0 = auto)

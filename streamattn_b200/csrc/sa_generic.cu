@@ -1,10 +1,11 @@
 // Generic CUDA-core decode kernel: any float dtype, any head_dim <= 256, any
 // strides / page size / layout.  It covers what the TMA + tensor-core streaming
 // kernel (sa_stream.cu) does not: fp32 caches, small or odd head sizes, tiny
-// pages, misaligned views.  One CTA handles one (row, query head, split); a
+// pages, misaligned views - and the same over 8-bit caches (CODE != kCodeNone: codes and
+// a scale byte a row, see sa_quant.cuh).  One CTA handles one (row, query head, split); a
 // second launch merges the split states exactly.  Also hosts the state-merge
 // kernel used after the cross-GPU gather of context-parallel decode.
-#include "sa_common.cuh"
+#include "sa_quant.cuh"
 
 namespace sa {
 
@@ -28,6 +29,7 @@ struct GenericParams {
     int32_t *trace;
     int splits;
     float scale_log2;
+    QuantScales quant;   // CODE != kCodeNone
 };
 
 // Element offset of virtual token t of (row b, kv head h); -1 when the page
@@ -52,7 +54,15 @@ __device__ inline int64_t token_offset(const SeqDesc &s, int b, int kvh, int64_t
     return page * s.pg_sp + (t % s.page_size) * s.pg_st + kvh * s.pg_sh;
 }
 
-template <typename T>
+// (K, V) scale bytes of virtual token t of an 8-bit cache; the token's page has been checked.
+__device__ inline uint32_t token_scales(const SeqDesc &s, const QuantScales &q, int b, int kvh, int64_t t, int64_t page)
+{
+    const int64_t outer = s.mode == kPaged ? page : b;
+    const int64_t tok = s.mode == kPaged ? t % s.page_size : t;
+    return reinterpret_cast<const uint16_t *>(q.scales)[outer * q.so + kvh * q.sh + tok];
+}
+
+template <typename T, int CODE>
 __global__ void __launch_bounds__(kGenericThreads)
 generic_partial_kernel(const __grid_constant__ GenericParams p)
 {
@@ -72,8 +82,9 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
     const int warp = threadIdx.x >> 5;
     if (!row_selected(p.seq, b)) return;  // row subset: this row is neither computed nor written
     const T *q = static_cast<const T *>(p.q) + b * p.q_sb + h * p.q_sh;
-    const T *kbase = static_cast<const T *>(p.k);
-    const T *vbase = static_cast<const T *>(p.v);
+    using KV = typename CacheElem<T, CODE>::type;
+    const KV *kbase = static_cast<const KV *>(p.k);
+    const KV *vbase = static_cast<const KV *>(p.v);
 
     for (int d = threadIdx.x; d < dim; d += kGenericThreads)
         sm_q[d] = Elem<T>::to_float(q[d]) * p.scale_log2;
@@ -89,13 +100,14 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
     float o[kMaxDim / 32];
 #pragma unroll
     for (int i = 0; i < kMaxDim / 32; ++i) o[i] = 0.0f;
+    bool nan_row = false;  // 8-bit caches: a token whose scale is NaN makes the result NaN
 
     for (int64_t blk = t_begin + warp * 32; blk < t_end; blk += kGenericWarps * 32) {
         const int64_t t = blk + lane;
         bool valid = t < t_end;
         int64_t off = -1;
+        int64_t page = -1;
         if (valid) {
-            int64_t page = -1;
             off = token_offset(p.seq, b, kvh, t, &page);
             if (off < 0) {
                 valid = false;
@@ -106,12 +118,21 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
             }
         }
         float s = -INFINITY;
+        float v_scale = 1.0f;
+        bool nan_scale = false;
         if (valid) {
-            const T *kr = kbase + off;
+            const KV *kr = kbase + off;
             float acc = 0.0f;
-            for (int d = 0; d < dim; ++d) acc = fmaf(sm_q[d], Elem<T>::to_float(kr[d]), acc);
+            for (int d = 0; d < dim; ++d) acc = fmaf(sm_q[d], CacheElem<T, CODE>::to_float(kr[d]), acc);
+            if (CODE != kCodeNone) {
+                const uint32_t pair = token_scales(p.seq, p.quant, b, kvh, t, page);
+                nan_scale = (pair & 0xffu) == kNanScaleByte || (pair >> 8) == kNanScaleByte;
+                acc = nan_scale ? 0.0f : acc * scale_value(pair & 0xffu);
+                v_scale = nan_scale ? 0.0f : scale_value(pair >> 8);
+            }
             s = acc;
         }
+        if (CODE != kCodeNone) nan_row = nan_row || __any_sync(0xffffffffu, nan_scale);
         const float blk_max = warp_max(s);
         if (blk_max == -INFINITY) continue;  // every token of the block was skipped
         const float m_new = fmaxf(m, blk_max);
@@ -121,14 +142,14 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
 #pragma unroll
         for (int i = 0; i < kMaxDim / 32; ++i) o[i] *= alpha;
         for (int j = 0; j < 32; ++j) {
-            const float pj = __shfl_sync(0xffffffffu, pr, j);
+            const float pj = __shfl_sync(0xffffffffu, CODE != kCodeNone ? pr * v_scale : pr, j);
             const int64_t offj = __shfl_sync(0xffffffffu, off, j);
             if (pj == 0.0f || offj < 0) continue;  // warp-uniform
-            const T *vr = vbase + offj;
+            const KV *vr = vbase + offj;
 #pragma unroll
             for (int i = 0; i < kMaxDim / 32; ++i) {
                 const int d = lane + 32 * i;
-                if (d < dim) o[i] = fmaf(pj, Elem<T>::to_float(vr[d]), o[i]);
+                if (d < dim) o[i] = fmaf(pj, CacheElem<T, CODE>::to_float(vr[d]), o[i]);
             }
         }
         m = m_new;
@@ -141,7 +162,8 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
 #pragma unroll
     for (int i = 0; i < kMaxDim / 32; ++i) {
         const int d = lane + 32 * i;
-        if (d < dim) sm_o[warp][d] = o[i];
+        // (m, l) stay finite, so the merge weighs the NaN in rather than dropping the state.
+        if (d < dim) sm_o[warp][d] = nan_row ? __uint_as_float(0x7fffffffu) : o[i];
     }
     __syncthreads();
 
@@ -238,7 +260,7 @@ merge_states_rows_kernel(const __grid_constant__ GenericParams p, int parts, int
     merge_row<T>(p.partials, parts, part_stride, row_stride, p.head_dim, p.out, p.out_mode, p.partials, row);
 }
 
-template <typename T>
+template <typename T, int CODE = kCodeNone>
 cudaError_t launch_generic_typed(const Problem &p, int splits, cudaStream_t stream)
 {
     GenericParams gp;
@@ -259,9 +281,10 @@ cudaError_t launch_generic_typed(const Problem &p, int splits, cudaStream_t stre
     gp.trace = p.trace;
     gp.splits = splits;
     gp.scale_log2 = kLog2e / sqrtf(static_cast<float>(p.head_dim));
+    gp.quant = p.quant;
     const int pairs = p.batch * p.q_heads;
     dim3 grid(splits, pairs);
-    generic_partial_kernel<T><<<grid, kGenericThreads, 0, stream>>>(gp);
+    generic_partial_kernel<T, CODE><<<grid, kGenericThreads, 0, stream>>>(gp);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess || splits == 1) return err;
     const int64_t stride = p.head_dim + 2;
@@ -269,6 +292,15 @@ cudaError_t launch_generic_typed(const Problem &p, int splits, cudaStream_t stre
     // would not do): reuse the descriptor inside the launch parameters of the first kernel.
     merge_states_rows_kernel<T><<<pairs, 128, 0, stream>>>(gp, splits, stride, stride * splits);
     return cudaGetLastError();
+}
+
+template <int CODE> cudaError_t launch_generic_quant(const Problem &p, int splits, cudaStream_t stream)
+{
+    switch (p.dtype) {
+        case SA_DTYPE_BF16: return launch_generic_typed<__nv_bfloat16, CODE>(p, splits, stream);
+        case SA_DTYPE_F16: return launch_generic_typed<__half, CODE>(p, splits, stream);
+        default: return launch_generic_typed<float, CODE>(p, splits, stream);
+    }
 }
 
 }  // namespace
@@ -292,6 +324,8 @@ size_t generic_partial_floats(int batch, int q_heads, int head_dim, int splits)
 
 cudaError_t launch_generic(const Problem &p, int splits, cudaStream_t stream)
 {
+    if (p.quant.code == kCodeE4M3) return launch_generic_quant<kCodeE4M3>(p, splits, stream);
+    if (p.quant.code == kCodeInt8) return launch_generic_quant<kCodeInt8>(p, splits, stream);
     switch (p.dtype) {
         case SA_DTYPE_BF16: return launch_generic_typed<__nv_bfloat16>(p, splits, stream);
         case SA_DTYPE_F16: return launch_generic_typed<__half>(p, splits, stream);

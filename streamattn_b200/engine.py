@@ -40,6 +40,8 @@ from .decode import (
     normalize_stream_attn_mode,
 )
 from .paged import PagedExactDecodePlan, PagedExactDecodeRunner, PagedKVCache
+from .quant_cache import QuantKVCache, QuantPagedKVCache
+from .quant_kv import QuantDecodePlan
 
 _Runner = Union[StreamAttnSeedOnlyDirectRunner, StreamAttnExactNativeDirectRunner, PagedExactDecodeRunner]
 
@@ -47,6 +49,11 @@ _PAGED_REASON = {
     STREAMATTN_MODE_EXACT_NATIVE: "explicit_paged_exact_native",
     STREAMATTN_MODE_VERIFIED_AUTO: "paged_kv_exact_only",
 }
+_QUANT_REASON = {
+    STREAMATTN_MODE_EXACT_NATIVE: "explicit_quant_exact_native",
+    STREAMATTN_MODE_VERIFIED_AUTO: "quant_kv_exact_only",
+}
+_QUANT_CACHES = (QuantKVCache, QuantPagedKVCache)
 
 
 @dataclass(frozen=True)
@@ -68,7 +75,7 @@ class StreamAttnEnginePlan:
     model_id: Optional[str]
     layer_id: Optional[int]
     query: torch.Tensor
-    key_cache: Union[torch.Tensor, PagedKVCache]
+    key_cache: Union[torch.Tensor, PagedKVCache, QuantKVCache, QuantPagedKVCache]
     value_cache: Optional[torch.Tensor]
     service: StreamAttnSeedOnlyDecodeService
     direct_runner: Optional[_Runner] = None
@@ -113,6 +120,25 @@ def _paged_serving_info(query: torch.Tensor, cache: PagedKVCache, plan: PagedExa
         runtime_counters=counters, stats=stats)
 
 
+def _quant_serving_info(query: torch.Tensor, cache: Union[QuantKVCache, QuantPagedKVCache], plan: QuantDecodePlan,
+                        reason: str) -> StreamAttnServingInfo:
+    """Telemetry record of an exact plan over an 8-bit cache."""
+
+    stats: Dict[str, Any] = {"layout": cache.normalized_layout, "code_dtype": str(cache.key.dtype).removeprefix("torch."),
+                             "splits": plan.splits, "workspace_bytes": plan.workspace_bytes}
+    if isinstance(cache, QuantPagedKVCache):
+        stats["page_size"] = cache.page_size
+        stats["max_pages_per_request"] = cache.max_pages_per_request
+    lens = cache.sequence_lengths
+    return StreamAttnServingInfo(
+        backend_used=plan.backend, plan_backend=plan.backend, plan_reason=reason,
+        policy_id=None, fallback_reason=None, model_id=None, layer_id=None,
+        batch_size=int(query.shape[0]), kv_len=cache.max_sequence_length if lens is None else int(lens.max().item()),
+        dtype=str(query.dtype).removeprefix("torch."), device=str(query.device),
+        seed_only_enabled=False, safety_policy_matched=False,
+        runtime_counters={"backend_counts": {plan.backend: 1}, "fallback_reasons": {}}, stats=stats)
+
+
 class StreamAttnEngine:
     """Plans and runs the native decode modes over caller-owned buffers."""
 
@@ -146,6 +172,14 @@ class StreamAttnEngine:
         info = _paged_serving_info(query, cache, plan, reason)
         return _Route(plan.backend, reason, PagedExactDecodeRunner(plan=plan, info=info))
 
+    def _quant_route(self, mode: str, query: torch.Tensor, cache: Union[QuantKVCache, QuantPagedKVCache]) -> _Route:
+        if mode not in _QUANT_REASON:
+            raise ValueError("seed_only_native does not support 8-bit KV; use exact_native or verified_auto")
+        plan = QuantDecodePlan.build(query, cache)
+        reason = _QUANT_REASON[mode]
+        info = _quant_serving_info(query, cache, plan, reason)
+        return _Route(plan.backend, reason, PagedExactDecodeRunner(plan=plan, info=info))
+
     def _resolve_route(self, mode: str, query, key_cache, value_cache, ids: Dict[str, Any]) -> _Route:
         if mode == STREAMATTN_MODE_EXACT_NATIVE:
             return self._exact_route("explicit_exact_native", query, key_cache, value_cache, ids)
@@ -160,20 +194,22 @@ class StreamAttnEngine:
 
     # -- public API ------------------------------------------------------------------------
 
-    def plan(self, query: torch.Tensor, key_cache: Union[torch.Tensor, PagedKVCache],
+    def plan(self, query: torch.Tensor,
+             key_cache: Union[torch.Tensor, PagedKVCache, QuantKVCache, QuantPagedKVCache],
              value_cache: Optional[torch.Tensor] = None, *, mode: str = STREAMATTN_MODE_VERIFIED_AUTO,
              model_id: Optional[str] = None, layer_id: Optional[int] = None) -> StreamAttnEnginePlan:
         """Check the call once, choose its route and bind it to the given buffers."""
 
         mode = normalize_stream_attn_mode(mode)
         paged = isinstance(key_cache, PagedKVCache)
-        if paged and value_cache is not None:
-            raise ValueError("value_cache must be omitted when key_cache is PagedKVCache")
-        if not paged and value_cache is None:
+        quant = isinstance(key_cache, _QUANT_CACHES)
+        if (paged or quant) and value_cache is not None:
+            raise ValueError(f"value_cache must be omitted when key_cache is {type(key_cache).__name__}")
+        if not (paged or quant) and value_cache is None:
             raise ValueError("value_cache is required for contiguous KV decode")
-        if paged:
+        if paged or quant:
             ids: Dict[str, Any] = {"model_id": None, "layer_id": None}
-            route = self._paged_route(mode, query, key_cache)
+            route = self._quant_route(mode, query, key_cache) if quant else self._paged_route(mode, query, key_cache)
         else:
             ids = {"model_id": self.service.model_id if model_id is None else model_id,
                    "layer_id": self.service.layer_id if layer_id is None else layer_id}

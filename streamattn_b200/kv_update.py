@@ -14,12 +14,13 @@ host synchronisation and can be captured in a CUDA graph.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import List, Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import native
 from .paged import PagedKVCache
+from .quant_cache import QuantPagedKVCache
 
 
 def _rows(t: torch.Tensor, heads_axis: int, name: str) -> Tuple[int, int, int, int, int]:
@@ -281,19 +282,21 @@ class PagePool:
 class PagedKVWriter:
     """Grows the requests of a :class:`PagedKVCache` token by token.
 
+    A :class:`QuantPagedKVCache` is grown the same way, also by several tokens at a time.
+
     Holds host mirrors of the lengths and of the pages each request owns, assigns a fresh page
     from the pool whenever a request's next token starts a new page (one small device write into
     ``cache.page_table``), and launches the append.  The device never waits for the host: page
     assignment for step ``t + 1`` can be enqueued while step ``t`` is still running.
     """
 
-    cache: PagedKVCache
+    cache: Union[PagedKVCache, QuantPagedKVCache]
     pool: PagePool
     lengths: List[int]
     pages: List[List[int]] = field(default_factory=list)
 
     @classmethod
-    def attach(cls, cache: PagedKVCache, pool: Optional[PagePool] = None) -> "PagedKVWriter":
+    def attach(cls, cache: Union[PagedKVCache, QuantPagedKVCache], pool: Optional[PagePool] = None) -> "PagedKVWriter":
         """Adopt a cache as it is (reads lengths and page table back once)."""
 
         lengths = [int(x) for x in cache.sequence_lengths.tolist()]
@@ -304,8 +307,9 @@ class PagedKVWriter:
             pool = PagePool(int(cache.key.shape[0]), reserved=[p for row in pages for p in row])
         return cls(cache=cache, pool=pool, lengths=lengths, pages=pages)
 
-    def reserve(self, tokens: int = 1) -> int:
-        """Make sure every request has pages for ``tokens`` more tokens; returns pages assigned.
+    def reserve(self, tokens: Union[int, Sequence[int]] = 1) -> int:
+        """Make sure every request has pages for ``tokens`` more tokens (one number, or one for each
+        request); returns pages assigned.
 
         All-or-nothing: every row's need is worked out and checked against the table capacity and
         the pool first, and only then are pages taken and the device table written, so a refused
@@ -315,8 +319,11 @@ class PagedKVWriter:
         page_size = self.cache.page_size
         max_pages = int(self.cache.page_table.shape[1])
         wanted: List[Tuple[int, int, int]] = []  # (row, pages it has, pages it needs)
+        more = [tokens] * len(self.lengths) if isinstance(tokens, int) else [int(x) for x in tokens]
+        if len(more) != len(self.lengths) or min(more, default=0) < 0:
+            raise ValueError("tokens must be one number, or one per request, and not negative")
         for b, n in enumerate(self.lengths):
-            need = -(-(n + tokens) // page_size)
+            need = -(-(n + more[b]) // page_size)
             if need > max_pages:
                 raise ValueError("sequence lengths exceed page_table capacity")
             if need > len(self.pages[b]):
@@ -342,11 +349,34 @@ class PagedKVWriter:
         return total
 
     def append(self, key_new: torch.Tensor, value_new: torch.Tensor, **kwargs) -> Optional[torch.Tensor]:
-        """Append one token to every request (assigning pages first); lengths advance on the device."""
+        """Append one token to every request (assigning pages first); lengths advance on the device.
 
+        An 8-bit cache takes any number of tokens, ``[B, T, Hkv, D]``; ``counts`` (a host sequence, one
+        entry per request) says how many of them are real.
+        """
+
+        if isinstance(self.cache, QuantPagedKVCache):
+            return self._append_quantized(key_new, value_new, **kwargs)
         self.reserve(1)
         out = paged_append_kv(self.cache, key_new, value_new, advance_lengths=True, **kwargs)
         self.lengths = [n + 1 for n in self.lengths]
+        return out
+
+    def _append_quantized(self, key_new: torch.Tensor, value_new: torch.Tensor, *, counts: Optional[Sequence[int]] = None,
+                          **kwargs) -> Optional[torch.Tensor]:
+        from .quant_kv import QuantizeKVPlan  # builds on this module
+
+        if not {"positions", "lengths_out", "advance_lengths"}.isdisjoint(kwargs):
+            raise ValueError("the writer chooses the positions and lengths itself")
+        tokens = int(key_new.shape[1 if _heads_axis(kwargs.get("new_layout", "BNHD")) == 2 else 2])
+        more = [tokens] * len(self.lengths) if counts is None else [int(x) for x in counts]
+        if len(more) != len(self.lengths) or any(not 0 <= n <= tokens for n in more):
+            raise ValueError("counts must hold one entry per request, between 0 and the number of new tokens")
+        on_device = None if counts is None else torch.tensor(more, dtype=torch.int32, device=self.cache.key.device)
+        plan = QuantizeKVPlan.build(self.cache, key_new, value_new, counts=on_device, **kwargs)  # checks before pages are taken
+        self.reserve(more)
+        out = plan.run()
+        self.lengths = [n + m for n, m in zip(self.lengths, more)]
         return out
 
     def release(self, row: int) -> None:

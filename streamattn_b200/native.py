@@ -25,6 +25,7 @@ SA_ERR_DEVICE = 4
 SA_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 SA_INDEX = {torch.int32: 0, torch.int64: 1}
 SA_LAYOUT = {"NHD": 0, "HND": 1}
+SA_KV_CODE = {torch.float8_e4m3fn: 1, torch.int8: 2}
 SA_BLOCK_ORDER = {"sequential": 0, "recent_first": 1, "sink_recent_first": 2}
 SA_OUT_FINAL = 0
 SA_OUT_STATE = 1
@@ -46,6 +47,18 @@ _sz = ctypes.c_size_t
 _i32p = ctypes.POINTER(ctypes.c_int32)
 _i64p = ctypes.POINTER(ctypes.c_int64)
 
+
+
+class QuantCacheStruct(ctypes.Structure):
+    """``sa_quant_cache_t``: an 8-bit KV cache, contiguous (``page_table`` null) or paged."""
+
+    _fields_ = [("key", _vp), ("value", _vp), ("scales", _vp), ("code", _i), ("batch", _i), ("kv_heads", _i),
+                ("head_dim", _i), ("capacity", _i64), ("stride_b", _i64), ("stride_n", _i64), ("stride_h", _i64),
+                ("scale_stride_b", _i64), ("scale_stride_h", _i64), ("page_table", _vp), ("table_dtype", _i),
+                ("page_size", _i), ("max_pages", _i), ("num_pages", _i64), ("layout", _i)]
+
+
+_QUANT_ARGS = [_vp, ctypes.POINTER(QuantCacheStruct), _vp, _vp, _sz, _vp, _i, _vp, _i, _i64, _i64, _i, _i, _i, _i]
 _EXACT_ARGS = [_vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i64,
                _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i]
 _PAGED_ARGS = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _i, _i, _i, _i64,
@@ -93,6 +106,15 @@ _SIGNATURES = {
     "sa_o_proj": ([_vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i, _i, _vp], _i),
     # k_new v_new k_cache v_cache | positions pos_dtype num_positions lens_out | cos sin rope_stride_b |
     # q_in q_out q_heads 4 q strides | batch kv_heads head_dim kv_len | 2 new strides | 3 kv strides | dtype status stream
+    "sa_quant_decode": (_QUANT_ARGS + [_vp], _i),
+    "sa_quant_plan_create": (_QUANT_ARGS, _vp),
+    # cache | k_new v_new tokens 3 strides | positions pos_dtype num_positions | counts counts_dtype | lens_out |
+    # cos sin 2 strides | q_in q_out q_heads 6 strides | dtype status stream
+    "sa_quantize_kv": ([ctypes.POINTER(QuantCacheStruct), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _i, _vp, _i, _vp,
+                        _vp, _vp, _i64, _i64, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp], _i),
+    # cache | k_out v_out tokens 3 strides | starts dtype | counts dtype | dtype status stream
+    "sa_dequantize_kv": ([ctypes.POINTER(QuantCacheStruct), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _i, _i,
+                          _vp, _vp], _i),
     "sa_append_kv": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _i64,
                       _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp], _i),
     # ... k_pages v_pages page_table table_dtype | positions ... | batch kv_heads head_dim page_size max_pages

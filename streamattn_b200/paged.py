@@ -164,6 +164,8 @@ class PagedExactDecodePlan:
         Triton path (``tokens_per_tile`` and friends) are accepted and ignored.
         """
 
+        if not isinstance(cache, PagedKVCache):
+            raise ValueError("cache must be a PagedKVCache (8-bit caches: QuantDecodePlan)")
         cache.validate(query, validate_metadata=validate_metadata)
         if output is None:
             output = torch.empty(query.shape, dtype=query.dtype, device=cache.key.device)
@@ -220,9 +222,9 @@ class PagedExactDecodePlan:
 
 @dataclass
 class PagedExactDecodeRunner:
-    """Engine-facing runner: a paged plan plus its precomputed telemetry."""
+    """Engine-facing runner: a plan over a cache record (paged, or 8-bit) plus its precomputed telemetry."""
 
-    plan: PagedExactDecodePlan
+    plan: Any
     info: Any
 
     def run(self) -> torch.Tensor:

@@ -1,0 +1,346 @@
+"""One-token attention over 8-bit KV caches, against the 64-bit oracle over the values the codes stand for.
+
+What may differ (all relative to sum_t p_t |v_t| unless said otherwise):
+  * the result is rounded to its type once: half a step of the value;
+  * p is rounded to fp16 before it meets the codes of V: 2^-11;
+  * a score is a sum of D products in fp32, some 2^-23 each of sum_d |q_d k_d| / sqrt(D), and a few more
+    roundings of that size; p = exp(score - max) carries the error of both, the denominator as well;
+  * the sums over N tokens in fp32: 2^-23 a step, and 2^-20 for the exponential.
+"""
+
+import pytest
+import torch
+
+import streamattn_b200 as sa
+from oracle import quant_kv as oracle
+from streamattn_b200 import native
+from tests.test_gpu_quant_kv import CODES, TYPES, dev, make_cache, new_rows  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+KERNELS = ["auto", "generic"]
+
+
+def tolerance(want, spread, reach, dtype, dim, tokens):
+    step = torch.finfo(dtype).eps / 2
+    inner = 2 ** -11 + 4 * (dim + 8) * 2 ** -23 * reach + tokens * 2 ** -23 + 2 ** -20
+    return step * want.abs() + spread * (1 + step) * inner + torch.finfo(dtype).tiny
+
+
+def check(got, q, mirror, lengths, rows=None):
+    want, spread, reach = oracle.attend(q, mirror, lengths)
+    tol = tolerance(want, spread, reach, q.dtype, q.shape[-1], max([int(n) for n in lengths] + [1]))
+    off = (got.cpu().double() - want).abs() - tol
+    rows = range(len(lengths)) if rows is None else rows
+    for b in rows:
+        assert bool((off[b] <= 0).all()), (b, int(lengths[b]), float(off[b].max()), float(want[b].abs().max()))
+
+
+def filled(dev, kind, layout, code, batch, heads, dim, capacity, lengths, page=16, seed=0, table_dtype=torch.int32, lens_dtype=torch.int32):
+    """A cache of random rows up to each row's length; behind it the codes and scales are random bytes, NaNs among them."""
+    cache, mirror = make_cache(dev, kind, layout, code, batch, heads, dim, capacity, page=page, seed=seed, table_dtype=table_dtype)
+    T = max(max(lengths), 1)
+    k, v = new_rows((batch, T, heads, dim), torch.float32, seed + 1), new_rows((batch, T, heads, dim), torch.float32, seed + 2)
+    k = k / k.square().mean(-1, keepdim=True).sqrt().clamp_min(1.0)        # scores of a few units
+    oracle.write(mirror, k, v, [0] * batch, lengths)
+    for name in ("key", "value", "scales"):
+        getattr(cache, name).view(torch.uint8).copy_(mirror[name].view(torch.uint8))
+    lens = torch.tensor(lengths, dtype=lens_dtype, device=dev)
+    fields = dict(key=cache.key, value=cache.value, scales=cache.scales, sequence_lengths=lens, layout=layout)
+    if kind == "paged":
+        return sa.QuantPagedKVCache(page_table=cache.page_table, **fields), mirror
+    return sa.QuantKVCache(**fields), mirror
+
+
+CASES = [
+    # kind, layout, code, dtype, kv_heads, group, dim, lengths, page
+    ("contig", "BHND", "e4m3", "bf16", 2, 8, 64, [300, 1, 0, 64], 0),
+    ("contig", "BNHD", "int8", "fp16", 2, 4, 128, [257, 65, 63], 0),
+    ("contig", "BHND", "int8", "bf16", 1, 16, 128, [190], 0),
+    ("contig", "BNHD", "e4m3", "fp16", 3, 1, 64, [129, 2], 0),
+    ("contig", "BHND", "e4m3", "bf16", 1, 24, 64, [100, 70], 0),          # a group that is split in two
+    ("paged", "HND", "e4m3", "bf16", 2, 8, 64, [300, 1, 0, 16, 17], 16),
+    ("paged", "NHD", "int8", "fp16", 2, 4, 128, [200, 64, 65], 64),
+    ("paged", "HND", "int8", "bf16", 1, 7, 128, [143, 9], 8),
+    ("paged", "NHD", "e4m3", "fp16", 2, 16, 64, [260, 128], 128),
+    ("paged", "HND", "e4m3", "fp16", 2, 2, 128, [130, 300], 32),
+    # the generic kernel's own ground: sizes, pages and types that have no tensor-core form
+    ("contig", "BHND", "int8", "fp32", 2, 2, 64, [70, 33], 0),
+    ("contig", "BNHD", "e4m3", "bf16", 2, 3, 80, [70, 33], 0),
+    ("contig", "BHND", "e4m3", "fp16", 1, 2, 256, [40], 0),
+    ("paged", "HND", "int8", "bf16", 2, 2, 64, [70, 33, 5], 4),
+    ("paged", "NHD", "e4m3", "fp32", 1, 2, 13, [70, 33, 5], 24),
+]
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_decode_matches_the_oracle(dev, case, kernel):
+    kind, layout, code, dtype, H, G, D, lengths, page = case
+    B = len(lengths)
+    cache, mirror = filled(dev, kind, layout, code, B, H, D, -(-max(lengths) // 8) * 8 + 8, lengths, page=page or 16, seed=D + G)
+    q = new_rows((B, 1, H * G, D), TYPES[dtype], 9).clamp(-30, 30)
+    plan = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel)
+    out = plan.run()
+    assert plan.device_status() == 0 and out is plan.output
+    check(out, q, mirror, lengths)
+    first = out.clone()
+    assert torch.equal(plan.run(), first)                                 # the same bits from launch to launch
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert not bool(out[b].any())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("splits", [1, 3, 40])
+def test_any_number_of_splits(dev, kernel, splits):
+    lengths = [700, 64, 130]
+    cache, mirror = filled(dev, "paged", "HND", "int8", 3, 2, 64, 1024, lengths, table_dtype=torch.int64, lens_dtype=torch.int64)
+    q = new_rows((3, 1, 8, 64), torch.bfloat16, 3).clamp(-30, 30)
+    plan = sa.QuantDecodePlan.build(q.to(dev), cache, splits=splits, kernel=kernel)
+    check(plan.run(), q, mirror, lengths)
+    dynamic = sa.QuantDecodePlan.build(q.to(dev), cache, splits=splits, kernel=kernel, dynamic_schedule=True)
+    check(dynamic.run(), q, mirror, lengths)
+    check(dynamic.run(), q, mirror, lengths)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("code", list(CODES))
+def test_scales_of_any_size(dev, kernel, code):
+    """Rows from 2^-90 to 2^90 next to each other: none may overflow, underflow or hide another."""
+    B, H, D, lengths = 2, 2, 64, [200, 130]
+    cache, mirror = filled(dev, "contig", "BHND", code, B, H, D, 256, lengths, seed=4)
+    g = torch.Generator().manual_seed(8)
+    e = torch.randint(37, 218, (B, H, 256), generator=g)
+    e[0, 0] = torch.randint(37, 60, (256,), generator=g)                   # a head of small values throughout
+    mirror["scales"][..., 1] = e.to(torch.uint8)
+    mirror["scales"][..., 0].clamp_(100, 120)
+    cache.scales.copy_(mirror["scales"])
+    q = new_rows((B, 1, 8, D), torch.bfloat16, 3).clamp(-2, 2)
+    q[1, 0, 0] *= 2.0 ** -100
+    q[1, 0, 1] *= 2.0 ** 40
+    got = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel).run()
+    check(got, q, mirror, lengths)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_nan_rows_reach_their_head_and_no_other(dev, kernel):
+    B, H, G, D, lengths = 3, 2, 4, 64, [200, 130, 64]
+    cache, mirror = filled(dev, "paged", "HND", "e4m3", B, H, D, 256, lengths, seed=6)
+    bad = torch.full((1, 1, H, D), 1.0)
+    bad[0, 0, 1, 5] = float("nan")                                         # K of head 1 of row 0, in the middle of the row
+    oracle_at = mirror["scales"]
+    page, slot = oracle.place(mirror, 0, 77)
+    oracle_at[page, 1, slot, 0] = 255
+    page, slot = oracle.place(mirror, 2, 63)
+    oracle_at[page, 0, slot, 1] = 255                                      # V of head 0 of row 2, its last token
+    page, slot = oracle.place(mirror, 1, 130)
+    oracle_at[page, :, slot] = 255                                         # behind row 1's last token
+    cache.scales.copy_(oracle_at)
+    q = new_rows((B, 1, H * G, D), torch.bfloat16, 3).clamp(-30, 30)
+    for splits in (None, 1, 5):
+        out = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel, splits=splits).run().cpu().view(B, H, G, D)
+        nan = torch.isnan(out)
+        assert bool(nan[0, 1].all()) and bool(nan[2, 0].all())
+        assert not bool(nan[0, 0].any()) and not bool(nan[2, 1].any()) and not bool(nan[1].any())
+    mirror["scales"][mirror["scales"] == 255] = 120
+    out = out.view(B, 1, H * G, D)
+    want, spread, reach = oracle.attend(q, mirror, lengths)
+    tol = tolerance(want, spread, reach, q.dtype, D, 200)
+    for b, h in ((0, 0), (1, 0), (1, 1), (2, 1)):
+        at = slice(h * G, (h + 1) * G)
+        assert bool(((out[b, 0, at].double() - want[b, 0, at]).abs() <= tol[b, 0, at]).all())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 64, 128])
+def test_bad_pages_are_left_out_and_reported(dev, kernel, page, dim):
+    B, H, lengths = 2, 2, [400, 300]
+    cache, mirror = filled(dev, "paged", "HND", "e4m3", B, H, dim, 512, lengths, page=page, seed=page)
+    pool = mirror["scales"].shape[0]
+    mirror["table"][0, 1], mirror["table"][1, 0], mirror["table"][0, 0] = -1, pool, 2 ** 31 - 1
+    mirror["table"][1, lengths[1] // page] = -(2 ** 31)
+    cache.page_table.copy_(mirror["table"])
+    with pytest.raises(ValueError, match="active page_table entries must reference physical pages"):
+        sa.QuantDecodePlan.build(torch.zeros(B, 1, 4, dim, dtype=torch.bfloat16, device=dev), cache)
+    q = new_rows((B, 1, 4, dim), torch.bfloat16, 3).clamp(-30, 30)
+    plan = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel, validate_metadata=False)
+    out = plan.run()
+    assert plan.device_status() == native.SA_DEV_BAD_PAGE
+    check(out, q, mirror, lengths)
+    cache.page_table.fill_(-1)                                             # nothing is left: zeros, as for an empty row
+    assert not bool(plan.run().any()) and plan.device_status() == native.SA_DEV_BAD_PAGE
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_row_subsets_states_and_page_walk(dev, kernel):
+    B, H, G, D, lengths = 4, 2, 4, 64, [200, 130, 64, 0]
+    cache, mirror = filled(dev, "paged", "NHD", "int8", B, H, D, 256, lengths, page=16, seed=2)
+    q = new_rows((B, 1, H * G, D), torch.bfloat16, 3).clamp(-30, 30)
+    out = torch.full((B, 1, H * G, D), 5.0, dtype=torch.bfloat16, device=dev)
+    rows = torch.tensor([2, 0, 2, 99], dtype=torch.int64, device=dev)
+    plan = sa.QuantDecodePlan.build(q.to(dev), cache, output=out, kernel=kernel, row_indices=rows, record_page_walk=True)
+    plan.run()
+    check(out, q, mirror, lengths, rows=[0, 2])
+    assert bool((out[[1, 3]] == 5.0).all())
+    plan.set_row_indices(None)
+    plan.run()
+    check(out, q, mirror, lengths)
+    walk = torch.full_like(mirror["table"], -1)
+    for b, n in enumerate(lengths):
+        walk[b, :-(-n // 16)] = mirror["table"][b, :-(-n // 16)]
+    assert torch.equal(plan.trace.cpu(), walk)
+    # states of the first 100 and of the other tokens merge to the whole
+    want, spread, reach = oracle.attend(q, mirror, lengths)
+    state = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel, return_state=True).run()
+    assert tuple(state.shape) == (B, H * G, D + 2) and state.dtype == torch.float32
+    o, l = state[..., :D].double().cpu(), state[..., D + 1].double().cpu()
+    assert l[3].tolist() == [0.0] * (H * G) and torch.isinf(state[3, :, D]).all()
+    tol = tolerance(want, spread, reach, torch.float32, D, 200)
+    assert bool(((o[:3] / l[:3, :, None] - want[:3, 0]).abs() <= tol[:3, 0]).all())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_lengths_change_on_the_device_and_graphs_follow(dev, kernel):
+    B, H, G, D = 2, 2, 4, 128
+    cache, mirror = filled(dev, "contig", "BHND", "e4m3", B, H, D, 512, [511, 511], seed=3)
+    q = new_rows((B, 1, H * G, D), torch.float16, 3).clamp(-30, 30)
+    plan = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel)
+    plan.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run()
+    for lengths in ([500, 400], [0, 511], [1, 0], [-3, 10 ** 6], [64, 128]):
+        cache.sequence_lengths.copy_(torch.tensor(lengths))
+        graph.replay()
+        clipped = [min(max(n, 0), 512) for n in lengths]
+        if max(clipped) < 512:
+            check(plan.output, q, mirror, clipped)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        plan.run()
+    side.synchronize()
+    check(plan.output, q, mirror, [64, 128])
+
+
+def test_two_plans_at_once(dev):
+    B, H, G, D = 4, 2, 8, 64
+    lengths = [4000, 3000, 10, 2000]
+    cache = sa.QuantKVCache.empty(B, H, 4096, D, device=dev)
+    k, v = torch.randn(B, 4096, H, D, device=dev).bfloat16(), torch.randn(B, 4096, H, D, device=dev).bfloat16()
+    sa.quantize_kv(cache, k, v, counts=torch.tensor(lengths, device=dev))
+    qs = [torch.randn(B, 1, H * G, D, device=dev).bfloat16() for _ in range(2)]
+    plans = [sa.QuantDecodePlan.build(q, cache) for q in qs]
+    alone = [p.run().clone() for p in plans]
+    streams = [torch.cuda.Stream(dev) for _ in plans]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, s in zip(plans, streams):
+            with torch.cuda.stream(s):
+                p.run()
+    torch.cuda.synchronize()
+    for p, want in zip(plans, alone):
+        assert torch.equal(p.output, want) and p.device_status() == 0
+
+
+def test_pinned_query_and_output(dev):
+    lengths = [200, 30]
+    cache, mirror = filled(dev, "contig", "BNHD", "int8", 2, 2, 64, 256, lengths, seed=3)
+    q = new_rows((2, 1, 8, 64), torch.bfloat16, 3).clamp(-30, 30).pin_memory()
+    out = torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16).pin_memory()
+    plan = sa.QuantDecodePlan.build(q, cache, output=out)
+    plan.run()
+    torch.cuda.synchronize()
+    check(out, q, mirror, lengths)
+
+
+def test_strided_query_and_views_of_larger_caches(dev):
+    B, H, G, D, lengths = 2, 2, 4, 64, [90, 33]
+    cache, mirror = filled(dev, "contig", "BHND", "e4m3", B, H, D, 96, lengths, seed=7)
+    q = new_rows((B, 1, H * G, 3 * D), torch.bfloat16, 3).clamp(-30, 30)
+    dq = q.to(dev)[..., D:2 * D]
+    check(sa.stream_attn_quant_decode(dq, cache), q[..., D:2 * D], mirror, lengths)
+    # odd capacity: rows of scales that start between the copies' boundaries
+    wide = {n: torch.zeros(B, H, 97, *tail, dtype=torch.uint8, device=dev) for n, tail in (("key", (D,)), ("value", (D,)), ("scales", (2,)))}
+    for n, t in wide.items():
+        t[:, :, :96].copy_(getattr(cache, n).view(torch.uint8))
+    odd = sa.QuantKVCache(key=wide["key"].view(torch.float8_e4m3fn), value=wide["value"].view(torch.float8_e4m3fn),
+                          scales=wide["scales"].view(torch.float8_e8m0fnu), sequence_lengths=cache.sequence_lengths)
+    check(sa.stream_attn_quant_decode(dq, odd), q[..., D:2 * D], mirror, lengths)
+
+
+@pytest.mark.parametrize("code", list(CODES))
+def test_serving_loop_prompt_steps_release_and_read_back(dev, code):
+    """The operators together: ragged prompts, decode steps with rotation, a request replaced, the history read back."""
+    B, H, G, D, page = 3, 2, 4, 64, 16
+    cache = sa.QuantPagedKVCache.empty(24, page, H, D, batch=B, max_pages_per_request=8, dtype=CODES[code], device=dev)
+    mirror = dict(key=cache.key.cpu(), value=cache.value.cpu(), scales=cache.scales.cpu(), table=None, page=page, capacity=8 * page,
+                  heads_first=True)
+    writer = sa.PagedKVWriter.attach(cache)
+    dtype, held, T = torch.bfloat16, [0] * B, 70
+
+    def update(tokens, counts, seed):
+        k, v = new_rows((B, tokens, H, D), dtype, seed), new_rows((B, tokens, H, D), dtype, seed + 1)
+        k = (k.float() / k.float().square().mean(-1, keepdim=True).sqrt().clamp_min(1.0)).to(dtype)
+        q = torch.randn(B, tokens, H * G, D, generator=torch.Generator().manual_seed(seed)).to(dtype)
+        at = torch.tensor(held)[:, None] + torch.arange(tokens)
+        angle = at[..., None].double() * 10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))
+        angle = torch.cat((angle, angle), -1)
+        cos, sin = angle.cos().to(dtype), angle.sin().to(dtype)
+        turned = writer.append(k.to(dev), v.to(dev), counts=counts, cos=cos.to(dev), sin=sin.to(dev), query=q.to(dev))
+        counts = counts or [tokens] * B
+        mirror["table"] = cache.page_table.cpu()
+        oracle.write(mirror, oracle.rotate(k, cos, sin), v, held, counts)
+        for b in range(B):
+            held[b] += counts[b]
+        want = oracle.rotate(q, cos, sin).to(dtype)
+        for b in range(B):
+            assert torch.equal(turned[b, :counts[b]].cpu(), want[b, :counts[b]])
+        return turned, want
+
+    update(T, [70, 33, 0], 1)
+    assert writer.lengths == held == cache.sequence_lengths.tolist()
+    query = torch.empty(B, 1, H * G, D, dtype=dtype, device=dev)
+    plan = sa.StreamAttnEngine().plan(query, cache, mode="exact_native")
+    for step in range(20):
+        turned, want = update(1, None, 10 + 2 * step)
+        query.copy_(turned)
+        out = plan.run(return_info=False)
+        check(out, want, mirror, held)
+    writer.release(1)
+    held[1] = 0
+    update(5, [0, 5, 0], 90)
+    assert writer.lengths == held == cache.sequence_lengths.tolist()
+    out, info = sa.decode(query, cache)
+    check(out, query.cpu(), mirror, held)
+    assert info.backend_used == plan.backend and info.plan_reason == "quant_kv_exact_only" and info.kv_len == max(held)
+    key, value = sa.dequantize_kv(cache, dtype=dtype, tokens=96)
+    for b in range(B):
+        k, v, _ = oracle.rows(mirror, b, 0, held[b])
+        assert torch.equal(key[b, :held[b]].cpu(), k.to(dtype)) and torch.equal(value[b, :held[b]].cpu(), v.to(dtype))
+        assert not bool(key[b, held[b]:].any()) and not bool(value[b, held[b]:].any())
+    # refused calls leave the writer, the table and the lengths as they were
+    before = (list(writer.lengths), cache.page_table.clone(), cache.sequence_lengths.clone(), writer.pool.free_pages)
+    k = torch.zeros(B, 100, H, D, dtype=dtype, device=dev)
+    for kwargs in (dict(), dict(counts=[101, 0, 0]), dict(counts=[1, 2]), dict(positions=cache.sequence_lengths)):
+        with pytest.raises(ValueError):
+            writer.append(k, k, **kwargs)
+    assert writer.lengths == before[0] and torch.equal(cache.page_table, before[1]) and torch.equal(cache.sequence_lengths, before[2])
+    assert writer.pool.free_pages == before[3]
+
+
+def test_engine_routes_over_contiguous_caches(dev):
+    lengths = [200, 30]
+    cache, mirror = filled(dev, "contig", "BNHD", "int8", 2, 2, 64, 256, lengths, seed=3)
+    q = new_rows((2, 1, 8, 64), torch.bfloat16, 3).clamp(-30, 30)
+    out, info = sa.decode(q.to(dev), cache, mode="exact_native")
+    check(out, q, mirror, lengths)
+    assert info.plan_reason == "explicit_quant_exact_native" and info.stats["code_dtype"] == "int8" and info.kv_len == 200
+    with pytest.raises(ValueError, match="must be omitted"):
+        sa.decode(q.to(dev), cache, cache.value)
+    with pytest.raises(ValueError, match="8-bit KV"):
+        sa.decode(q.to(dev), cache, mode="seed_only_native")
+    full = sa.QuantKVCache(key=cache.key, value=cache.value, scales=cache.scales.clamp(100, 120), layout="BNHD")
+    assert sa.decode(q.to(dev), full)[1].kv_len == 256
