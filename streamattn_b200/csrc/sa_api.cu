@@ -102,27 +102,29 @@ EncodeTiledFn encode_fn()
     return fn;
 }
 
-// 4-D map (column, x1, x2, outer) over a bf16/f16 cache with 128-byte swizzled boxes
-// of 64 columns x `box_tokens` tokens; tok_dim says which of x1/x2 is the token axis.
-bool encode_map(CUtensorMap *map, int dtype, const void *base, const uint64_t dims[4], const uint64_t strides[3],
+// 4-D map (column, x1, x2, outer) over a cache; tok_dim says which of x1/x2 is the token axis.
+// bf16/f16: 128-byte swizzled boxes of 64 columns x `box_tokens` tokens.  8-bit codes: boxes of a whole
+// row (64 or 128 columns) x `box_tokens`, swizzled over its 64 or 128 bytes.
+bool encode_map(CUtensorMap *map, int dtype, bool quant, const void *base, const uint64_t dims[4], const uint64_t strides[3],
                 int tok_dim, int box_tokens)
 {
     EncodeTiledFn fn = encode_fn();
     if (fn == nullptr) return false;
     if (reinterpret_cast<uintptr_t>(base) % 16) return false;
     cuuint64_t gdim[4] = {dims[0], dims[1], dims[2], dims[3]};
-    cuuint64_t gstr[3] = {strides[0] * 2, strides[1] * 2, strides[2] * 2};
+    const cuuint64_t size = quant ? 1 : 2;
+    cuuint64_t gstr[3] = {strides[0] * size, strides[1] * size, strides[2] * size};
     for (int i = 0; i < 4; ++i)
         if (gdim[i] == 0 || gdim[i] > (1ull << 32)) return false;
     for (int i = 0; i < 3; ++i)
         if (gstr[i] == 0 || gstr[i] % 16 || gstr[i] >= (1ull << 40)) return false;
-    cuuint32_t box[4] = {64, 1, 1, 1};
+    cuuint32_t box[4] = {quant ? static_cast<cuuint32_t>(dims[0]) : 64, 1, 1, 1};
     box[tok_dim] = static_cast<cuuint32_t>(box_tokens);
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    const CUtensorMapDataType dt =
-        dtype == SA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapDataType dt = quant ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : dtype == SA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUresult rc = fn(map, dt, 4, const_cast<void *>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     quant && dims[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return rc == CUDA_SUCCESS;
 }
@@ -150,20 +152,20 @@ bool build_stream_geometry(const Problem &p, int64_t max_vlen, StreamGeometry *g
 {
     *why = "";
     if (p.dtype != SA_DTYPE_BF16 && p.dtype != SA_DTYPE_F16) { *why = "dtype is not bf16/fp16"; return false; }
-    if (p.quant.code != kCodeNone) { *why = "8-bit cache"; return false; }
+    const bool quant = p.quant.code != kCodeNone;
     if (p.head_dim != 64 && p.head_dim != 128) { *why = "head_dim is not 64 or 128"; return false; }
     geo->kv_split = stream_kv_split(p.q_heads / p.kv_heads);
     if (geo->kv_split == 0) { *why = "query heads per KV head cannot be split into groups of at most 16"; return false; }
     const int group = p.q_heads / p.kv_heads / geo->kv_split;  // per virtual KV head
     if (p.batch > 8192) { *why = "batch larger than 8192"; return false; }
-    if (stream_smem_bytes(p.head_dim, group > 8, stream_stages(p.head_dim, group > 8), p.batch) > kStreamSmemLimit) {
+    if (stream_smem_bytes(p.head_dim, group > 8, stream_stages(p.head_dim, group > 8, quant), p.batch, quant) > kStreamSmemLimit) {
         *why = "batch too large for the shared-memory schedule table";
         return false;
     }
     if (reinterpret_cast<uintptr_t>(p.q) % 4 || p.q_sb % 2 || p.q_sh % 2) { *why = "query not 4-byte aligned"; return false; }
     if (reinterpret_cast<uintptr_t>(p.out) % 16) { *why = "output not 16-byte aligned"; return false; }
     if (max_vlen <= 0 || max_vlen >= (1ll << 31)) { *why = "sequence length out of range"; return false; }
-    const int tile = stream_tile_tokens(p.head_dim);
+    const int tile = stream_tile_tokens(p.head_dim, quant);
     const SeqDesc &s = p.seq;
     const uint64_t D = static_cast<uint64_t>(p.head_dim);
     uint64_t dims[4];
@@ -203,13 +205,21 @@ bool build_stream_geometry(const Problem &p, int64_t max_vlen, StreamGeometry *g
             geo->tok_dim = 2;
         }
     }
+    if (quant) {
+        // Scale bytes move in untiled copies of whole fragments: 16-byte addresses and sizes.
+        if (reinterpret_cast<uintptr_t>(p.quant.scales) % 16 || p.quant.so % 8 || p.quant.sh % 8 ||
+            (s.mode == kContig && s.kv_len % 8)) {
+            *why = "scales of a row do not start and end on 16-byte boundaries";
+            return false;
+        }
+    }
     geo->frag_tokens = std::min(unit, tile);
     geo->frags_per_tile = tile / geo->frag_tokens;
     geo->frags_per_unit = s.mode == kContig ? 1 : std::max(1, unit / geo->frag_tokens);
     const bool uniform = s.mode == kBlocks || (s.mode == kContig && s.seq_lens == nullptr);
     geo->uniform_tiles = uniform ? static_cast<int>((max_vlen + tile - 1) / tile) : -1;
-    if (!encode_map(&geo->map_k, p.dtype, p.k, dims, strides, geo->tok_dim, geo->frag_tokens) ||
-        !encode_map(&geo->map_v, p.dtype, p.v, dims, strides, geo->tok_dim, geo->frag_tokens)) {
+    if (!encode_map(&geo->map_k, p.dtype, quant, p.k, dims, strides, geo->tok_dim, geo->frag_tokens) ||
+        !encode_map(&geo->map_v, p.dtype, quant, p.v, dims, strides, geo->tok_dim, geo->frag_tokens)) {
         *why = "cache pointers/strides do not satisfy the TMA alignment rules";
         return false;
     }

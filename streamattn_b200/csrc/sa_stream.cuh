@@ -13,6 +13,17 @@ constexpr int kStreamWarps = SA_STREAM_WARPS;    // each with its own ring of ti
 #define SA_STREAM_STAGES 1
 #endif
 constexpr int kStreamStages = SA_STREAM_STAGES;  // 16 KB K+V tiles in flight per warp
+#ifndef SA_QUANT_STAGES_64
+#define SA_QUANT_STAGES_64 2
+#endif
+constexpr int kQuantTileTokens = 64;             // 8-bit caches: 8 KB (D64) or 16 KB (D128) K+V tiles
+
+// Tiles in flight per warp: 16 KB of them, one where 16 head rows at D128 take 33 KB of state areas.
+constexpr int stages_of(int head_dim, bool rows16, bool quant)
+{
+    if (quant) return head_dim == 64 ? SA_QUANT_STAGES_64 : 1;
+    return (head_dim == 128 && rows16 && kStreamStages > 2) ? 2 : kStreamStages;
+}
 
 constexpr int kCpMaxWorld = SA_CP_MAX_WORLD;
 constexpr int kCpFuseWorld = 8;  // ranks the fused decode+exchange launch supports (one NVSwitch box)
@@ -53,10 +64,17 @@ struct StreamGeometry {
 // Smallest s with group % s == 0 and group / s <= 16 (0 if there is none): a KV head with more
 // than 16 query heads is served as s virtual KV heads that read the same K/V rows.
 int stream_kv_split(int group);
-int stream_tile_tokens(int head_dim);
-int stream_stages(int head_dim, bool rows16);
-size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch);
+int stream_tile_tokens(int head_dim, bool quant);
+int stream_stages(int head_dim, bool rows16, bool quant);
+size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch, bool quant);
 constexpr size_t kStreamSmemLimit = 227 * 1024 - 64;
+
+// The instances over 8-bit caches, in translation units of their own.
+struct StreamParams;
+cudaError_t launch_stream_e4m3(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int dtype, int head_dim,
+                               int ctas, cudaStream_t stream);
+cudaError_t launch_stream_int8(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int dtype, int head_dim,
+                               int ctas, cudaStream_t stream);
 cudaError_t launch_stream(const Problem &p, const StreamGeometry &geo, const CpFuse &cp, cudaStream_t stream);
 
 }  // namespace sa
