@@ -299,7 +299,7 @@ int finish_plan(sa_plan *plan, void *workspace, size_t workspace_bytes, int64_t 
         plan->use_stream = build_stream_geometry(p, max_vlen, &plan->geo, &why);
         if (!plan->use_stream && kernel_choice == SA_KERNEL_STREAM)
             return fail(SA_ERR_UNSUPPORTED, "streaming kernel does not cover this call: %s", why);
-        if (plan->use_stream && dynamic) plan->geo.schedule = kScheduleClaims;
+        if (plan->use_stream && dynamic && p.quant.code == kCodeNone) plan->geo.schedule = kScheduleClaims;
     }
     size_t need;
     if (plan->use_stream) {

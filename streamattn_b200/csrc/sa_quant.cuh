@@ -49,12 +49,15 @@ template <int CODE> __device__ __forceinline__ uint32_t encode4(float a, float b
     }
 }
 
-// Two codes in the low 16 bits of `x` to two halves (exact: 4 and 8 significant bits, |code| <= 448).
-__device__ __forceinline__ uint32_t e4m3x2_to_halves(uint32_t x)
+// Four e4m3 codes to two pairs of halves (exact: 4 significant bits, |code| <= 448).
+__device__ __forceinline__ void e4m3x4_to_halves(uint32_t x, uint32_t &lo, uint32_t &hi)
 {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
-    return r;
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(x));
 }
 
 // Four codes to two pairs of halves.  int8: with the sign bit flipped a byte is x + 128, and the
@@ -62,8 +65,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_halves(uint32_t x)
 template <int CODE> __device__ __forceinline__ void decode4(uint32_t codes, uint32_t &lo, uint32_t &hi)
 {
     if constexpr (CODE == kCodeE4M3) {
-        lo = e4m3x2_to_halves(codes);
-        hi = e4m3x2_to_halves(codes >> 16);
+        e4m3x4_to_halves(codes, lo, hi);
     } else {
         const uint32_t u = codes ^ 0x80808080u;
         const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
@@ -78,7 +80,8 @@ template <int CODE> __device__ __forceinline__ void decode4(uint32_t codes, uint
 template <int CODE> __device__ __forceinline__ float decode1(uint8_t code)
 {
     if constexpr (CODE == kCodeE4M3) {
-        const uint32_t h = e4m3x2_to_halves(code);
+        uint32_t h, unused;
+        e4m3x4_to_halves(code, h, unused);
         return __low2float(*reinterpret_cast<const __half2 *>(&h));
     } else {
         return static_cast<float>(static_cast<int8_t>(code));

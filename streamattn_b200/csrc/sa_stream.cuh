@@ -13,15 +13,24 @@ constexpr int kStreamWarps = SA_STREAM_WARPS;    // each with its own ring of ti
 #define SA_STREAM_STAGES 1
 #endif
 constexpr int kStreamStages = SA_STREAM_STAGES;  // 16 KB K+V tiles in flight per warp
-#ifndef SA_QUANT_STAGES_64
-#define SA_QUANT_STAGES_64 2
+#ifndef SA_QUANT_TILE
+#define SA_QUANT_TILE 64
 #endif
-constexpr int kQuantTileTokens = 64;             // 8-bit caches: 8 KB (D64) or 16 KB (D128) K+V tiles
+constexpr int kQuantTileTokens = SA_QUANT_TILE;  // 8-bit caches: 8 KB (D64) or 16 KB (D128) of codes a tile
+#ifndef SA_QUANT_STAGES
+#define SA_QUANT_STAGES(D) (128 / (D))
+#endif
+#ifndef SA_QUANT_WARPS
+#define SA_QUANT_WARPS 8
+#endif
+constexpr int kQuantWarps = SA_QUANT_WARPS;
 
-// Tiles in flight per warp: 16 KB of them, one where 16 head rows at D128 take 33 KB of state areas.
+constexpr int warps_of(bool quant) { return quant ? kQuantWarps : kStreamWarps; }
+
+// Tiles in flight per warp (the state areas of 16 head rows at D128 leave room for fewer).
 constexpr int stages_of(int head_dim, bool rows16, bool quant)
 {
-    if (quant) return head_dim == 64 ? SA_QUANT_STAGES_64 : 1;
+    if (quant) return SA_QUANT_STAGES(head_dim);
     return (head_dim == 128 && rows16 && kStreamStages > 2) ? 2 : kStreamStages;
 }
 

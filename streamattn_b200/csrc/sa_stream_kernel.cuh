@@ -23,9 +23,9 @@
 
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
-#include "sa_quant.cuh"
-#include "sa_stream.cuh"
+#include "sa_stream_quant.cuh"
 
 namespace sa {
 
@@ -167,33 +167,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
         : "memory");
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr)
+// True on one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one()
 {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint2 lds64(uint32_t addr)
-{
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint32_t lds32(uint32_t addr)
-{
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v)
-{
-    asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+    uint32_t chosen;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(chosen));
+    return chosen != 0u;
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3)
@@ -634,10 +617,11 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *scale_ring = ring + WARPS * STAGES * STAGE_BYTES;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(scale_ring + WARPS * STAGES * SCALE_BYTES);
+    uint8_t *scale_floats = scale_ring + WARPS * STAGES * SCALE_BYTES;       // the scales of a warp's current tile as floats
+    uint64_t *bars = reinterpret_cast<uint64_t *>(scale_floats + (QUANT ? WARPS * TILE_N * 8 : 0));
     float *states = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(bars) + BAR_BYTES);
     uint64_t *cp_stage = reinterpret_cast<uint64_t *>(states + WARPS * STATE_FLOATS);  // context-parallel: rows to send
-    float *scratch = reinterpret_cast<float *>(cp_stage + STATE_FLOATS);  // merges: 6 floats per thread
+    float *scratch = reinterpret_cast<float *>(cp_stage + (QUANT ? 0 : STATE_FLOATS));  // merges: 6 floats per thread
     int *prefix = reinterpret_cast<int *>(scratch + NTHREADS * 6);         // ragged rows: tiles before row b
     int *vlens = prefix + p.batch + 1;                                     // ragged rows: length of row b (-1: not selected)
     __shared__ int s_last;
@@ -655,6 +639,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 
     const uint32_t ring_u32 = smem_u32(ring) + warp * STAGES * STAGE_BYTES;
     const uint32_t scale_u32 = smem_u32(scale_ring) + warp * STAGES * SCALE_BYTES;
+    const uint32_t float_u32 = smem_u32(scale_floats) + warp * TILE_N * 8;
     const uint32_t bar_u32 = smem_u32(bars) + warp * STAGES * 8;
     uint8_t *warp_ring = ring + warp * STAGES * STAGE_BYTES;
 
@@ -809,7 +794,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 al_nseg = static_cast<int>(n_eff);
                 al_start = static_cast<int>(t0);
                 al_end = static_cast<int>(t1);
-                const bool claims = p.schedule == kScheduleClaims;
+                const bool claims = !QUANT && p.schedule == kScheduleClaims;
                 if ((claims || p.schedule == kScheduleCyclic) && n_eff == n_p && tiles_p >= n_p * WARPS * (STAGES + 1)) {
                     // Shared schedules: the pair's warps take tiles round-robin by position - all of
                     // them (cyclic), or only their first STAGES + 1, after which every tile is claimed
@@ -931,8 +916,17 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     };
     // Next tile of this warp's sequence (-1: none).  A claim is consumed one call after it was
     // issued, so the counter's round trip overlaps a whole tile of work.
+    // 8-bit caches: a tile holds half the bytes, so what is done once a tile weighs twice as much.  Their tiles
+    // come in steps of a constant (there is no dynamic schedule), and positions are 32-bit integers.
+    int step_x = dyn ? al_start + dyn_gw : lo + warp;
+    const int step = dyn ? dyn_nw : WARPS, step_end = dyn ? al_end : hi;
     auto next_tile = [&]() -> int {
         int x = -1;
+        if constexpr (QUANT) {
+            x = step_x < step_end ? step_x : -1;
+            step_x += step;
+            return x;
+        }
         if (!dyn) {
             if (seq_i < n_w) x = lo + warp + seq_i * WARPS;
         } else if (seq_i <= STAGES || !dyn_claims) {
@@ -967,12 +961,14 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     // the cursor only moves when a tile crosses into the next pair.
     int pc_b = -1, pc_kvh = 0, pc_start = 0, pc_end = 0;
     int64_t pc_vlen = 0;
+    int pc_head = 0;  // 8-bit caches: the cache's own head index of pc_kvh
     if (aligned && hi > lo) {  // all of this CTA's tiles belong to one pair: no search needed
         pc_b = al_pair / Hkv;
         pc_kvh = al_pair - pc_b * Hkv;
         pc_start = al_start;
         pc_end = al_end;
         pc_vlen = vlen_of(pc_b);
+        pc_head = pc_kvh / p.kv_split;
     }
     auto lookup = [&](int x) -> Frag {
         Frag f;
@@ -984,6 +980,26 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             pc_end = pc_start + row_tiles;
             if (b != pc_b) pc_vlen = vlen_of(b);
             pc_b = b;
+            pc_head = pc_kvh / p.kv_split;
+        }
+        if constexpr (QUANT) {
+            f.kvh = pc_head;
+            const int tok = (x - pc_start) * TILE_N + (lane << p.frag_shift);
+            const bool mine = lane < p.frags_per_tile && tok < static_cast<int>(pc_vlen);
+            f.tok = tok;
+            f.outer = pc_b;
+            f.state = mine;
+            if (p.seq.mode == kPaged && mine) {
+                const int page_shift = p.fpu_shift + p.frag_shift;
+                const int lp = tok >> page_shift;
+                const int64_t slot = static_cast<int64_t>(pc_b) * p.seq.max_pages + lp;
+                const int64_t page = load_index(p.seq.page_table, p.seq.table_i64, slot);
+                f.tok = tok - (lp << page_shift);
+                f.outer = static_cast<int>(page);
+                f.state = (page >= 0 && page < p.seq.num_pages) ? 1 : 2;
+                if (pc_kvh == 0 && f.tok == 0) f.trace_idx = slot;
+            }
+            return f;
         }
         f.kvh = p.kv_split > 1 ? pc_kvh / p.kv_split : pc_kvh;  // the cache's own head index
         if (lane >= p.frags_per_tile) return f;
@@ -1031,22 +1047,40 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if (f.state == 2) atomicOr(p.status, SA_DEV_BAD_PAGE);
         if (ok && p.trace != nullptr && f.trace_idx >= 0) p.trace[f.trace_idx] = static_cast<int32_t>(f.outer);
         const unsigned mask = __ballot_sync(0xffffffffu, ok);
-        constexpr int BOX_ROW = QUANT ? D : 128;  // bytes of one box row
-        // Scale bytes of a fragment: a page has them all, a contiguous row ends at the cache's capacity
-        // (its fragment is the whole tile, on lane 0).
-        uint32_t scale_bytes = 0;
         if constexpr (QUANT) {
-            const int64_t room = p.seq.kv_len - f.tok;
-            scale_bytes = 2 * (p.seq.mode == kContig && room < p.frag_tokens ? static_cast<uint32_t>(room) : p.frag_tokens);
+            // One elected lane issues the fragments one after the other: copies take their operands from uniform
+            // registers, and a lane each (below) is served by a loop over the lanes for every one of the
+            // three copies (measured with pages of 16, four fragments a tile: 39.3 instead of 40.6 us for 136 MB).
+            const unsigned bad = __ballot_sync(0xffffffffu, f.state == 2);
+            const bool leader = elect_one();
+            const int frag = p.frag_tokens;
+            int scale_bytes = 2 * frag;  // of a fragment: a page has them all, a row ends at the cache's capacity
+            if (p.seq.mode == kContig) {
+                const int room = static_cast<int>(p.seq.kv_len) - (f.tok - lane * frag);  // lane 0's fragment
+                scale_bytes = 2 * (room < frag ? room : frag);
+            }
+            if (leader) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(__popc(mask) * (frag * D * 2 + scale_bytes)));
+            for (unsigned left = mask; left != 0u; left &= left - 1) {
+                const int i = __ffs(left) - 1;
+                const int tok = __shfl_sync(0xffffffffu, f.tok, i);
+                const int outer = __shfl_sync(0xffffffffu, f.outer, i);
+                if (leader) {
+                    const uint32_t dst = stage + i * frag * D;
+                    const int c1 = p.tok_dim == 1 ? tok : f.kvh;
+                    const int c2 = p.tok_dim == 1 ? f.kvh : tok;
+                    tma_load_4d(dst, &tm_k, bar, 0, c1, c2, outer, policy);
+                    tma_load_4d(dst + TILE_BYTES, &tm_v, bar, 0, c1, c2, outer, policy);
+                    bulk_load(scale_u32 + slot * SCALE_BYTES + i * frag * 2,
+                              p.quant.scales + 2 * (outer * p.quant.so + f.kvh * p.quant.sh + tok), scale_bytes, bar, policy);
+                }
+            }
+            return bad;
         }
         if (lane == 0)
-            mbar_arrive_expect_tx(bar, static_cast<uint32_t>(__popc(mask)) * (p.frag_tokens * BOX_ROW * HALVES * 2 + scale_bytes));
+            mbar_arrive_expect_tx(bar, static_cast<uint32_t>(__popc(mask)) * p.frag_tokens * 128 * HALVES * 2);
         __syncwarp();
         if (ok) {
-            if constexpr (QUANT)
-                bulk_load(scale_u32 + slot * SCALE_BYTES + lane * p.frag_tokens * 2,
-                          p.quant.scales + 2 * (f.outer * p.quant.so + f.kvh * p.quant.sh + f.tok), scale_bytes, bar, policy);
-            const uint32_t dst = stage + lane * p.frag_tokens * BOX_ROW;
+            const uint32_t dst = stage + lane * p.frag_tokens * 128;
             const int c1 = p.tok_dim == 1 ? f.tok : f.kvh;
             const int c2 = p.tok_dim == 1 ? f.kvh : f.tok;
 #pragma unroll
@@ -1055,7 +1089,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 tma_load_4d(dst + TILE_BYTES + hf * HALF_BYTES, &tm_v, bar, hf * 64, c1, c2, f.outer, policy);
             }
         }
-        return QUANT ? __ballot_sync(0xffffffffu, f.state == 2) : 0u;
+        return 0u;
     };
 
     // Rows of one length: the dependency wait (see the note at launch_dependents) comes here, or
@@ -1122,46 +1156,10 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 
         // Query fragments of this KV group (A operand of q.k), rows >= group are zero.
         uint32_t qa[KS_QK][4];
-        float row_scale[2] = {p.scale_log2, p.scale_log2};  // what turns a row's products into base-2 scores
+        QuantWarp<T, D, QUANT ? TILE_N : 32, ROWS16, QUANT ? CODE : kCodeInt8> qw;  // 8-bit caches: all of the warp's arithmetic
         if constexpr (QUANT) {
-            // 8-bit caches: the operands are halves whatever T is, the codes being exact in that type.  A row
-            // of q is multiplied by the power of two that brings its largest element to [2^14, 2^15): exact
-            // for all but elements some 2^30 times smaller than that one, and undone by row_scale.
-            // The order of the k index is the one the codes are loaded in (see the tile loop): k-step
-            // 4 * j + s holds columns base + 4 * s + {0, 1} and + {2, 3} of the lane's j-th 16 bytes.
-            const T *qrow[2];
-            qrow[0] = static_cast<const T *>(p.q) + b * p.q_sb + (static_cast<int64_t>(kvh) * group + g) * p.q_sh;
-            qrow[1] = qrow[0] + 8 * p.q_sh;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const bool ok = r == 0 ? g < group : ROWS16 && g + 8 < group;
-                float x[KS_QK][4];
-                float big = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < KS_QK; ++ks) {
-                    const int col = (D == 128 ? 2 * t4 + (ks >> 2) : t4) * 16 + (ks & 3) * 4;
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const uint32_t w = ok ? *reinterpret_cast<const uint32_t *>(qrow[r] + col + e) : 0u;
-                        const T *pair = reinterpret_cast<const T *>(&w);
-                        x[ks][e] = Elem<T>::to_float(pair[0]);
-                        x[ks][e + 1] = Elem<T>::to_float(pair[1]);
-                        big = fmaxf(big, fmaxf(fabsf(x[ks][e]), fabsf(x[ks][e + 1])));
-                    }
-                }
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                // Exponent of the factor: at least -114, and at most 100 to keep row_scale clear of zero.
-                int up = 14 - (static_cast<int>(__float_as_uint(big) >> 23) - 127);
-                up = big > 0.0f ? (up < 100 ? up : 100) : 0;
-                const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-                row_scale[r] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-#pragma unroll
-                for (int ks = 0; ks < KS_QK; ++ks) {
-                    qa[ks][r] = Mma<__half>::pack(x[ks][0] * factor, x[ks][1] * factor);
-                    qa[ks][2 + r] = Mma<__half>::pack(x[ks][2] * factor, x[ks][3] * factor);
-                }
-            }
+            qw.begin(static_cast<const T *>(p.q) + b * p.q_sb + static_cast<int64_t>(kvh) * group * p.q_sh, p.q_sh, group,
+                     p.scale_log2, g, t4);
         } else {
             const T *qrow0 = static_cast<const T *>(p.q) + b * p.q_sb + (static_cast<int64_t>(kvh) * group + g) * p.q_sh;
             const T *qrow1 = qrow0 + 8 * p.q_sh;
@@ -1179,10 +1177,6 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 
         float m_run[2] = {-INFINITY, -INFINITY};
         float l_run[2] = {0.0f, 0.0f};
-        // 8-bit caches: o_acc is kept in units of 2^(v_exp - 142), v_exp the largest scale byte of V so far
-        // (at least 16), and a NaN scale turns the segment's result into NaN.
-        int v_exp = 16;
-        bool nan_scale = false;
         float o_acc[NT_O][4];
 #pragma unroll
         for (int i = 0; i < NT_O; ++i) {
@@ -1195,6 +1189,40 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         for (;; ++j) {
             const int x = xq[0];
             if (x < 0 || x >= seg_end) break;
+            if constexpr (QUANT) {
+                const int at = (j % STAGES);
+                if (!__all_sync(0xffffffffu, mbar_try_wait(bar_u32 + at * 8, (j / STAGES) & 1u))) {  // not there yet
+                    if (!dead && !mbar_wait(bar_u32 + at * 8, (j / STAGES) & 1u, p.wait_ns)) {
+                        dead = true;
+                        atomicOr(p.status, SA_DEV_PIPELINE_TIMEOUT);
+                    }
+                    dead = __any_sync(0xffffffffu, dead);
+                    if (dead) {  // as below
+#pragma unroll
+                        for (int s = 0; s < STAGES; ++s) xq[s] = -1;
+                        pending.x = -1;
+                        step_x = step_end;
+                        break;
+                    }
+                }
+                const int left = static_cast<int>(vlen) - (x - pair_start) * TILE_N;
+                const uint32_t kb = ring_u32 + at * STAGE_BYTES;
+                qw.tile(kb, kb + TILE_BYTES, scale_u32 + at * SCALE_BYTES, float_u32, left < TILE_N ? left : TILE_N, badq[0],
+                        p.frag_shift, lane, g, t4);
+                fence_proxy_async();  // as below
+                __syncwarp();
+                unsigned left_out = 0u;
+                if (pending.x >= 0) left_out = issue(j + STAGES, pending);
+#pragma unroll
+                for (int s = 0; s + 1 < STAGES; ++s) {
+                    xq[s] = xq[s + 1];
+                    badq[s] = badq[s + 1];
+                }
+                xq[STAGES - 1] = pending.x;
+                badq[STAGES - 1] = left_out;
+                pending = lookup(next_tile());
+                continue;
+            }
             const int lt = x - pair_start;
             const uint32_t slot = static_cast<uint32_t>(j) % STAGES;
             const uint32_t parity = (static_cast<uint32_t>(j) / STAGES) & 1u;
@@ -1219,184 +1247,6 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const int n_valid = vlen - tile_tok0 < TILE_N ? static_cast<int>(vlen - tile_tok0) : TILE_N;
             const bool tail = n_valid < TILE_N;
 
-            if constexpr (QUANT) {
-                // 8-bit caches.  The operands of both products are halves: the codes are exact in that type, q was
-                // scaled into it, and p is weighted with the token's V scale before it is rounded to it.
-                //
-                // Lane (g, t4) owns token column g of a score tile and reads its K row in 16-byte pieces, whose bytes
-                // 4s .. 4s+3 are the lane's elements of k-step s: a dot product does not mind the order of its terms,
-                // and q was arranged to match.  A V row is read in pieces of D/8 bytes, dimensions g*D/8 ..: output
-                // tile i takes the i-th byte of every lane's piece.  Which token a column stands for is chosen
-                // so that no two lanes of a load phase meet in a bank under the copies' swizzle: tokens in order
-                // for D = 128; for D = 64, whose 128-byte lines hold two tokens, columns 2t and 2t + 1 of a tile
-                // are tokens x(t) = {0, 1, 4, 5} and x(t) ^ 3.
-                const uint32_t sb = scale_u32 + slot * SCALE_BYTES;
-                const unsigned bad = badq[0];
-                const bool partial = tail || bad != 0u;
-                auto valid = [&](int tok) { return tok < n_valid && ((bad >> (tok >> p.frag_shift)) & 1u) == 0u; };
-                uint32_t pairs = lds32(sb + lane * 4);  // (K, V) bytes of tokens 2 * lane and 2 * lane + 1
-                if (partial) {
-                    // Tokens behind the row's end or on a page that is not there: what the buffers hold
-                    // for them is stale.  Their V codes and scale bytes become zeros, their scores -inf below.
-                    if (!valid(2 * lane)) pairs &= 0xffff0000u;
-                    if (!valid(2 * lane + 1)) pairs &= 0x0000ffffu;
-                    uint8_t *vtile = warp_ring + slot * STAGE_BYTES + TILE_BYTES;
-                    for (int i = lane; i < TILE_N * (D / 16); i += 32)
-                        if (!valid(i / (D / 16))) *reinterpret_cast<uint4 *>(vtile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                const uint32_t is_nan = __vcmpeq4(pairs, 0xffffffffu);
-                pairs &= ~is_nan;
-                const int my_top = static_cast<int>(max((pairs >> 8) & 0xffu, pairs >> 24));
-                int top = __reduce_max_sync(0xffffffffu, is_nan != 0u ? 256 : my_top);
-                const bool has_nan = top == 256;
-                if (has_nan) {
-                    nan_scale = true;
-                    top = __reduce_max_sync(0xffffffffu, my_top);
-                }
-                if (partial || has_nan) {
-                    sts32(sb + lane * 4, pairs);
-                    __syncwarp();
-                }
-                const int old_exp = v_exp;
-                v_exp = v_exp > top ? v_exp : top;
-
-                const int tok_lo = D == 128 ? 2 * t4 : (t4 & 1) | ((t4 & 2) << 1);  // token of column 2 * t4 of a tile
-                const int tok_hi = D == 128 ? tok_lo + 1 : tok_lo ^ 3;              // ... and of column 2 * t4 + 1
-                const int tok_g = D == 128 ? g : ((g >> 1) & 1) | (g & 4);          // token of column g
-                const int k_row = D == 128 || (g & 1) == 0 ? tok_g : tok_g ^ 3;
-
-                float s_acc[NT_S][4];
-                uint32_t w[NT_S];  // K, V bytes of the lane's two tokens of a tile
-                float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-                for (int nt = 0; nt < NT_S; ++nt) {
-                    if constexpr (D == 128) {
-                        w[nt] = lds32(sb + (nt * 8 + 2 * t4) * 2);
-                    } else {
-                        const uint2 four = lds64(sb + (nt * 8 + (t4 >> 1) * 4) * 2);  // tokens 4 * (t4 / 2) ..
-                        w[nt] = __byte_perm(four.x, four.y, (t4 & 1) ? 0x5432 : 0x7610);
-                    }
-                    s_acc[nt][0] = s_acc[nt][1] = s_acc[nt][2] = s_acc[nt][3] = 0.0f;
-                    const int row = nt * 8 + k_row;
-#pragma unroll
-                    for (int j16 = 0; j16 < D / 64; ++j16) {
-                        const int chunk = D == 128 ? (2 * t4 + j16) ^ (row & 7) : t4 ^ ((row >> 1) & 3);
-                        const uint4 c = lds128(kb + row * D + chunk * 16);
-                        const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            uint32_t b0, b1;
-                            decode4<CODE>(words[s], b0, b1);
-                            Mma<__half>::run(s_acc[nt], qa[j16 * 4 + s], b0, b1);
-                        }
-                    }
-                    const float k_lo = __uint_as_float((w[nt] << 23) & 0x7f800000u);
-                    const float k_hi = __uint_as_float((w[nt] << 7) & 0x7f800000u);
-                    s_acc[nt][0] *= k_lo;
-                    s_acc[nt][1] *= k_hi;
-                    if (ROWS16) {
-                        s_acc[nt][2] *= k_lo;
-                        s_acc[nt][3] *= k_hi;
-                    }
-                    if (partial) {
-                        if (!valid(nt * 8 + tok_lo)) s_acc[nt][0] = s_acc[nt][2] = -INFINITY;
-                        if (!valid(nt * 8 + tok_hi)) s_acc[nt][1] = s_acc[nt][3] = -INFINITY;
-                    }
-                    mx0 = fmaxf(mx0, fmaxf(s_acc[nt][0], s_acc[nt][1]));
-                    if (ROWS16) mx1 = fmaxf(mx1, fmaxf(s_acc[nt][2], s_acc[nt][3]));
-                }
-
-                // Online softmax; the running maximum is kept in the products' own unit and subtracted before
-                // row_scale is applied, so that the largest p is exactly 1 however large the scores are (with
-                // fma(s, scale, -max * scale) it is 2^(rounding of max * scale)).  p is multiplied by the V scale relative to the unit,
-                // 2^(e - v_exp + 15) <= 2^15: at the top of fp16's range, so that a small p or a small row of V
-                // keeps its eleven bits for another 2^29 below the largest.
-                uint32_t pa[KS_PV][4];
-                {
-                    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-                    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-                    const float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);
-                    const float m_new0 = fmaxf(m_run[0], mx0);
-                    const float sub0 = m_new0 == -INFINITY ? 0.0f : m_new0;
-                    const float alpha0 = exp2f((m_run[0] - sub0) * row_scale[0]);
-                    float m_new1 = -INFINITY, alpha1 = 0.0f, sub1 = 0.0f;
-                    if (ROWS16) {
-                        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-                        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-                        m_new1 = fmaxf(m_run[1], mx1);
-                        sub1 = m_new1 == -INFINITY ? 0.0f : m_new1;
-                        alpha1 = exp2f((m_run[1] - sub1) * row_scale[1]);
-                    }
-                    const int off = (142 - v_exp) * (1 << 23);
-                    float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-                    for (int nt = 0; nt < NT_S; ++nt) {
-                        const float v_lo = __int_as_float(max(static_cast<int>((w[nt] << 15) & 0x7f800000u) + off, 0));
-                        const float v_hi = __int_as_float(max(static_cast<int>((w[nt] >> 1) & 0x7f800000u) + off, 0));
-                        const float p0 = exp2f((s_acc[nt][0] - sub0) * row_scale[0]);
-                        const float p1 = exp2f((s_acc[nt][1] - sub0) * row_scale[0]);
-                        sum0 += p0 + p1;
-                        const int kt = nt >> 1;
-                        const int hi_half = (nt & 1) * 2;
-                        pa[kt][hi_half] = Mma<__half>::pack(p0 * v_lo, p1 * v_hi);
-                        pa[kt][hi_half + 1] = 0u;
-                        if (ROWS16) {
-                            const float p2 = exp2f((s_acc[nt][2] - sub1) * row_scale[1]);
-                            const float p3 = exp2f((s_acc[nt][3] - sub1) * row_scale[1]);
-                            sum1 += p2 + p3;
-                            pa[kt][hi_half + 1] = Mma<__half>::pack(p2 * v_lo, p3 * v_hi);
-                        }
-                    }
-                    l_run[0] = l_run[0] * alpha0 + sum0;
-                    m_run[0] = m_new0;
-                    const float o_alpha0 = alpha0 * unit, o_alpha1 = alpha1 * unit;
-                    if (ROWS16) {
-                        l_run[1] = l_run[1] * alpha1 + sum1;
-                        m_run[1] = m_new1;
-                    }
-#pragma unroll
-                    for (int i = 0; i < NT_O; ++i) {
-                        o_acc[i][0] *= o_alpha0;
-                        o_acc[i][1] *= o_alpha0;
-                        if (ROWS16) {
-                            o_acc[i][2] *= o_alpha1;
-                            o_acc[i][3] *= o_alpha1;
-                        }
-                    }
-                }
-
-                // O[16 rows, D] += P V: the two tokens of a lane's column pair come from two rows and are
-                // interleaved byte by byte, so that a conversion yields one operand register.
-#pragma unroll
-                for (int kt = 0; kt < KS_PV; ++kt) {
-                    uint32_t lo[2][D / 32], hi[2][D / 32];  // codes of the pair's two tokens, for k halves 0 and 1
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int row0 = (2 * kt + half) * 8 + tok_lo, row1 = (2 * kt + half) * 8 + tok_hi;
-                        if constexpr (D == 128) {
-                            const uint4 a = lds128(vb + row0 * D + ((g ^ (row0 & 7)) << 4));
-                            const uint4 c = lds128(vb + row1 * D + ((g ^ (row1 & 7)) << 4));
-                            lo[half][0] = a.x; lo[half][1] = a.y; lo[half][2] = a.z; lo[half][3] = a.w;
-                            hi[half][0] = c.x; hi[half][1] = c.y; hi[half][2] = c.z; hi[half][3] = c.w;
-                        } else {
-                            const uint2 a = lds64(vb + row0 * D + (((g >> 1) ^ ((row0 >> 1) & 3)) << 4) + (g & 1) * 8);
-                            const uint2 c = lds64(vb + row1 * D + (((g >> 1) ^ ((row1 >> 1) & 3)) << 4) + (g & 1) * 8);
-                            lo[half][0] = a.x; lo[half][1] = a.y;
-                            hi[half][0] = c.x; hi[half][1] = c.y;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        uint32_t b0[4], b1[4];
-                        decode4<CODE>(__byte_perm(lo[0][i], hi[0][i], 0x5140), b0[0], b0[1]);
-                        decode4<CODE>(__byte_perm(lo[0][i], hi[0][i], 0x7362), b0[2], b0[3]);
-                        decode4<CODE>(__byte_perm(lo[1][i], hi[1][i], 0x5140), b1[0], b1[1]);
-                        decode4<CODE>(__byte_perm(lo[1][i], hi[1][i], 0x7362), b1[2], b1[3]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) Mma<__half>::run(o_acc[4 * i + e], pa[kt], b0[e], b1[e]);
-                    }
-                }
-            } else {
             // scores: S[16 rows = heads, TILE_N tokens] = Q K^T
             float s_acc[NT_S][4];
 #pragma unroll
@@ -1515,26 +1365,22 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     Mma<T>::run(o_acc[2 * dp + 1], pa[kt], r2, r3);
                 }
             }
-            }
 
             // Order this warp's shared-memory accesses before the async-proxy writes of the refill.
             fence_proxy_async();
             __syncwarp();
-            unsigned left_out = 0u;
-            if (pending.x >= 0) left_out = issue(j + STAGES, pending);
+            if (pending.x >= 0) issue(j + STAGES, pending);
 #pragma unroll
-            for (int s = 0; s + 1 < STAGES; ++s) {
-                xq[s] = xq[s + 1];
-                badq[s] = badq[s + 1];
-            }
+            for (int s = 0; s + 1 < STAGES; ++s) xq[s] = xq[s + 1];
             xq[STAGES - 1] = pending.x;
-            badq[STAGES - 1] = left_out;
             pending = lookup(next_tile());
         }
 
         SA_STAMP(3);
         // Warp state -> the warp's state area: [ROWS][D+2] floats = (o, m, l).
-        {
+        if constexpr (QUANT) {
+            qw.store(states + warp * STATE_FLOATS, STATE_STRIDE, g, t4);
+        } else {
             l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], 1);
             l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], 2);
             if (ROWS16) {
@@ -1542,28 +1388,13 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 l_run[1] += __shfl_xor_sync(0xffffffffu, l_run[1], 2);
             }
             float *area = states + warp * STATE_FLOATS;
-            if constexpr (QUANT) {
-                // Column n of output tile i is dimension n * D/8 + i (see the tile loop).
-                const float unit = __uint_as_float(static_cast<uint32_t>(v_exp - 15) << 23);  // 2^(v_exp - 142)
 #pragma unroll
-                for (int i = 0; i < NT_O; ++i) {
-#pragma unroll
-                    for (int e = 0; e < (ROWS16 ? 4 : 2); ++e)
-                        area[(g + (e >> 1) * 8) * STATE_STRIDE + (2 * t4 + (e & 1)) * (D / 8) + i] =
-                            nan_scale ? __uint_as_float(0x7fffffffu) : o_acc[i][e] * unit;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < (QUANT ? 0 : NT_O); ++i) {
+            for (int i = 0; i < NT_O; ++i) {
                 const int d = i * 8 + 2 * t4;
                 *reinterpret_cast<float2 *>(area + g * STATE_STRIDE + d) = make_float2(o_acc[i][0], o_acc[i][1]);
                 if (ROWS16)
                     *reinterpret_cast<float2 *>(area + (g + 8) * STATE_STRIDE + d) =
                         make_float2(o_acc[i][2], o_acc[i][3]);
-            }
-            if constexpr (QUANT) {  // to base-2 scores, the unit of the states
-                m_run[0] *= row_scale[0];
-                m_run[1] *= row_scale[1];
             }
             if (t4 == 0) {
                 area[g * STATE_STRIDE + D] = m_run[0];
@@ -1783,9 +1614,10 @@ template <typename T, int D, int CODE>
 cudaError_t launch_dim(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int ctas, int batch,
                        bool rows16, cudaStream_t stream)
 {
+    constexpr bool kQuant = CODE != kCodeNone;
     if (rows16)
-        return launch_instance<T, D, kStreamWarps, stages_of(D, true, CODE != kCodeNone), true, CODE>(mk, mv, sp, ctas, batch, stream);
-    return launch_instance<T, D, kStreamWarps, stages_of(D, false, CODE != kCodeNone), false, CODE>(mk, mv, sp, ctas, batch, stream);
+        return launch_instance<T, D, warps_of(kQuant), stages_of(D, true, kQuant), true, CODE>(mk, mv, sp, ctas, batch, stream);
+    return launch_instance<T, D, warps_of(kQuant), stages_of(D, false, kQuant), false, CODE>(mk, mv, sp, ctas, batch, stream);
 }
 
 template <int CODE>

@@ -1,0 +1,485 @@
+// What the streaming kernel does with a tile of an 8-bit cache: the query's operand registers, the
+// products and the online softmax of one warp.  Used by stream_decode_kernel (sa_stream_kernel.cuh),
+// which moves the tiles.
+//
+//   S^T[token, head] = K q^T          tokens on the M rows of the tensor-core instructions, heads on N
+//   O^T[dim, head]  += V^T P^T
+//
+// e4m3   q is multiplied by the power of two that brings its largest element to [2^14, 2^15) and becomes fp16:
+//        exact for all but elements some 2^30 times smaller than that one.  The codes of K are converted to fp16, in
+//        which they are exact, and the products accumulate in fp32.  (There is an instruction with e4m3
+//        operands, but on this GPU it executes as conversions and fp16 products: measured 10 instructions
+//        and 16 cycles of the tensor pipe for its 16 x 8 x 32, where two fp16 instructions take the same.)
+// int8   the 8-bit integer instruction is native and twice as fast as fp16, so the codes of K go from shared
+//        memory into it as they are: q is scaled to integers of at most 32512 = 127 * 256 and split into two bytes,
+//        hi * 256 + lo, off by 2^-17 of the row's largest element; products and sums are exact in int32.
+// P V uses fp16 for both: p has a far larger range than two bytes hold (the tail of a long row may carry all of
+// its weight at 2^-20 of the maximum a token), and the codes are exact in fp16.
+//
+// Every score is then multiplied by the token's K scale, 2^e exactly.  p is multiplied by the V scale
+// relative to a unit, 2^(e - v_exp + 15) <= 2^15 with v_exp the largest V byte so far: at the top of fp16's
+// range, where a small p or a small row of V keeps its eleven bits down to 2^-29 of the largest.
+#pragma once
+
+#include <type_traits>
+#include <utility>
+
+#include "sa_quant.cuh"
+#include "sa_stream.cuh"
+
+namespace sa {
+namespace {
+
+// Shared-memory loads at a register plus a constant, which the instruction adds itself.
+template <int OFFSET> __device__ __forceinline__ uint4 lds128(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr), "n"(OFFSET)
+                 : "memory");
+    return v;
+}
+
+template <int OFFSET> __device__ __forceinline__ uint2 lds64(uint32_t addr)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(addr), "n"(OFFSET) : "memory");
+    return v;
+}
+
+template <int OFFSET> __device__ __forceinline__ uint32_t lds32(uint32_t addr)
+{
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(v) : "r"(addr), "n"(OFFSET) : "memory");
+    return v;
+}
+
+template <int OFFSET> __device__ __forceinline__ float2 lds_float2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2 + %3];" : "=f"(v.x), "=f"(v.y) : "r"(addr), "n"(OFFSET) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void sts_float4(uint32_t addr, float a, float b, float c, float d)
+{
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+__device__ __forceinline__ void sts128_zero(uint32_t addr)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+}
+
+// FIRST: c is the product alone, not added to.
+template <bool FIRST> __device__ __forceinline__ void mma_int8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (FIRST)
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// f(std::integral_constant<int, 0>) ... f(std::integral_constant<int, N - 1>): an unrolled loop whose index
+// is a constant expression.
+template <int N, typename F, int... I> __device__ __forceinline__ void unrolled(F &&f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void unrolled(F &&f)
+{
+    unrolled<N>(static_cast<F &&>(f), std::make_integer_sequence<int, N>{});
+}
+
+template <bool FIRST>
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if constexpr (FIRST)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four 8 x 16-byte matrices; lane i gives the address of row i % 8 of matrix i / 8.
+template <int OFFSET> __device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr), "n"(OFFSET)
+                 : "memory");
+}
+
+// Transposes an 8 x 8 matrix of halves, two of a row's elements a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack_halves(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Which tokens a lane meets.  A 16-token tile's rows r and r + 8 are the neighbours tile_token(r) and
+// tile_token(r) ^ 1, and lane (g, t4)'s columns 2 t4, 2 t4 + 1 of the second product are the four tokens
+// 4 t4 .. 4 t4 + 3 in an order that depends on t4.  Both are chosen so that no two lanes of a load phase meet
+// in a bank under the copies' swizzle: for D = 64 a 128-byte line holds two tokens and its 16-byte pieces are
+// permuted with bits 1-2 of the token, for D = 128 with bits 0-2.
+template <int D> __device__ __forceinline__ int token_flip(int t4) { return D == 64 ? (t4 ^ (t4 >> 1)) & 1 : t4 & 2; }
+template <int D> __device__ __forceinline__ int tile_token(int r) { return 4 * (r >> 1) + (((r & 1) * 3) ^ token_flip<D>(r >> 1)); }
+
+// Byte offset of 16-byte piece `chunk` of tile row `row`.
+template <int D> __device__ __forceinline__ uint32_t piece(int row, int chunk)
+{
+    return row * D + ((D == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4);
+}
+
+template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp {
+    static constexpr int NH = ROWS16 ? 2 : 1;     // groups of eight heads
+    static constexpr int SUB = TILE_N < 64 ? TILE_N : 64;  // tokens whose scores are held at a time
+    static constexpr int MT = SUB / 16;           // ... in 16-token tiles
+    static constexpr int PER_LANE = TILE_N / 32;  // tokens whose scales a lane prepares
+    static constexpr int KS = D / 32;             // k-steps of 32 dimensions
+    static constexpr int DT = D / 16;             // output tiles
+
+    // Operand registers of a k-step.  e4m3: two of each of its two fp16 instructions; int8: two of the high, two of the low bytes.
+    uint32_t q[NH][KS][4];
+    float row_scale[NH][2];      // heads 2 t4 and 2 t4 + 1: what turns the products into base-2 scores
+    float m[NH][2], l[NH][2];    // running maximum (in the products' unit) and this lane's part of the sum
+    float o[NH][DT][4];          // in units of 2^(v_exp - 142)
+    int v_exp;                   // largest scale byte of V so far, at least 16
+    bool has_nan;                // a NaN scale was met: the result is NaN
+
+    // Query rows of `group` heads from head0 on; lane (g, t4) holds columns of head g of each eight.
+    __device__ __forceinline__ void begin(const T *q0, int64_t stride, int group, float scale_log2, int g, int t4)
+    {
+        v_exp = 16;
+        has_nan = false;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+            const bool ok = nh * 8 + g < group;
+            const T *row = q0 + (nh * 8 + g) * stride;
+            float x[KS][8];
+            uint32_t amax = 0;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const int col = 32 * ks + 4 * t4 + (e >> 2) * 16 + (e & 2);
+                    const uint32_t w = ok ? *reinterpret_cast<const uint32_t *>(row + col) : 0u;
+                    const T *pair = reinterpret_cast<const T *>(&w);
+                    x[ks][e] = Elem<T>::to_float(pair[0]);
+                    x[ks][e + 1] = Elem<T>::to_float(pair[1]);
+                    amax = max(amax, max(__float_as_uint(x[ks][e]) & 0x7fffffffu, __float_as_uint(x[ks][e + 1]) & 0x7fffffffu));
+                }
+            }
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            float scale;
+            if constexpr (CODE == kCodeE4M3) {
+                // Exponent of the factor: at least -113, and at most 100 to keep the scale clear of zero.
+                const int up = amax == 0 ? 0 : min(14 + 127 - static_cast<int>(amax >> 23), 100);
+                const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+                scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu)   // a NaN or an infinity: NaN
+                                            : scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+                // A 32-bit word of K codes c0 .. c3 becomes the halves c0 c1 and c2 c3; a lane's word 4 t4 .. of the first
+                // 16 bytes of a k-step meets the lane's word of the second 16 bytes in one instruction each.
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    q[nh][ks][0] = pack_halves(x[ks][0] * factor, x[ks][1] * factor);
+                    q[nh][ks][1] = pack_halves(x[ks][4] * factor, x[ks][5] * factor);
+                    q[nh][ks][2] = pack_halves(x[ks][2] * factor, x[ks][3] * factor);
+                    q[nh][ks][3] = pack_halves(x[ks][6] * factor, x[ks][7] * factor);
+                }
+            } else {
+                const float big = fmaxf(__uint_as_float(amax), __uint_as_float(27u << 23));
+                const float inv = 32512.0f / big;
+                scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : scale_log2 * (big * (1.0f / 32512.0f));
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        int hi[4], lo[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int v = max(min(__float2int_rn(x[ks][half * 4 + i] * inv), 32512), -32512);
+                            hi[i] = (v + 128) >> 8;
+                            lo[i] = v - hi[i] * 256;
+                        }
+                        q[nh][ks][half] = bytes4(hi);
+                        q[nh][ks][2 + half] = bytes4(lo);
+                    }
+            }
+            row_scale[nh][0] = __shfl_sync(0xffffffffu, scale, 8 * t4);
+            row_scale[nh][1] = __shfl_sync(0xffffffffu, scale, 8 * t4 + 4);
+            m[nh][0] = m[nh][1] = -INFINITY;
+            l[nh][0] = l[nh][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.0f;
+        }
+    }
+
+    __device__ __forceinline__ static uint32_t bytes4(const int (&v)[4])
+    {
+        return __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
+    }
+
+    // One tile: codes at kb and vb, scale pairs at sb, room for TILE_N float pairs at fb (shared memory).
+    // Tokens from n_valid on, and those of the fragments in `bad` (1 << frag_shift tokens each), are not there.
+    __device__ __forceinline__ void tile(uint32_t kb, uint32_t vb, uint32_t sb, uint32_t fb, int n_valid, unsigned bad,
+                                         int frag_shift, int lane, int g, int t4)
+    {
+        const bool partial = n_valid < TILE_N || bad != 0u;
+        auto valid = [&](int tok) { return tok < n_valid && ((bad >> (tok >> frag_shift)) & 1u) == 0u; };
+
+        // The scale bytes become floats once a token: K's as it is, V's relative to the unit.  Tokens that are not
+        // there get zeros, and so do their V codes: what the buffers hold for them is stale.
+        uint32_t pairs[PER_LANE / 2];
+        if constexpr (PER_LANE == 4) {
+            const uint2 x = lds64<0>(sb + lane * 8);
+            pairs[0] = x.x;
+            pairs[PER_LANE / 2 - 1] = x.y;
+        } else {
+            pairs[0] = lds32<0>(sb + lane * 4);
+        }
+        if (partial) {
+#pragma unroll
+            for (int i = 0; i < PER_LANE / 2; ++i) {
+                if (!valid(PER_LANE * lane + 2 * i)) pairs[i] &= 0xffff0000u;
+                if (!valid(PER_LANE * lane + 2 * i + 1)) pairs[i] &= 0x0000ffffu;
+            }
+            for (int i = lane; i < TILE_N * (D / 16); i += 32)
+                if (!valid(i / (D / 16))) sts128_zero(vb + i * 16);
+        }
+        uint32_t my_top = 0, nan_bytes = 0;
+#pragma unroll
+        for (int i = 0; i < PER_LANE / 2; ++i) {
+            const uint32_t nan = __vcmpeq4(pairs[i], 0xffffffffu);
+            pairs[i] &= ~nan;
+            nan_bytes |= nan;
+            my_top = max(my_top, max((pairs[i] >> 8) & 0xffu, pairs[i] >> 24));
+        }
+        int top = static_cast<int>(__reduce_max_sync(0xffffffffu, nan_bytes != 0u ? 256u : my_top));
+        if (top == 256) {
+            has_nan = true;
+            top = static_cast<int>(__reduce_max_sync(0xffffffffu, my_top));
+        }
+        const int old_exp = v_exp;
+        v_exp = max(v_exp, top);
+        const int off = (142 - v_exp) * (1 << 23);
+#pragma unroll
+        for (int i = 0; i < PER_LANE / 2; ++i) {
+            const float k0 = __uint_as_float((pairs[i] << 23) & 0x7f800000u), k1 = __uint_as_float((pairs[i] << 7) & 0x7f800000u);
+            const float v0 = __int_as_float(max(static_cast<int>((pairs[i] << 15) & 0x7f800000u) + off, 0));
+            const float v1 = __int_as_float(max(static_cast<int>((pairs[i] >> 1) & 0x7f800000u) + off, 0));
+            sts_float4(fb + (PER_LANE * lane + 2 * i) * 8, k0, v0, k1, v1);
+        }
+        __syncwarp();
+        float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);
+
+        // Every 16-token tile has the same swizzle, so a lane's places in it are computed once a tile.
+        const int row_g = tile_token<D>(g);
+        const uint32_t f0 = fb + row_g * 8, f1 = fb + (row_g ^ 1) * 8;
+        // K, matrix loads: matrices 0 and 2 are rows 0-7 of a 16-token tile, 1 and 3 rows 8-15; 0 and 1 are the first
+        // 16 bytes of a k-step, 2 and 3 the second.
+        const uint32_t k_at = piece<D>(tile_token<D>(lane & 7) ^ ((lane >> 3) & 1), lane >> 4);
+        // V: the tokens of the lane's columns are tok, tok ^ 3 | tok ^ 1, tok ^ 2; D/8 bytes of each.
+        const int tok = 4 * t4 + token_flip<D>(t4);
+        uint32_t v_at[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int row = tok ^ (c == 0 ? 0 : c == 1 ? 3 : c == 2 ? 1 : 2);
+            v_at[c] = vb + (D == 128 ? piece<D>(row, g) : piece<D>(row, g >> 1) + (g & 1) * 8);
+        }
+
+#pragma unroll 1
+        for (int first = 0; first < TILE_N; first += SUB) {
+            if (first >= n_valid) break;
+            float s[MT][NH][4];
+            float v_weight[MT][2];
+            uint32_t k_from[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) k_from[ks] = kb + first * D + (k_at ^ (ks << 5));
+            unrolled<MT>([&](auto mt_c) {
+                constexpr int mt = decltype(mt_c)::value;
+                [[maybe_unused]] int hi[NH][4], lo[NH][4];
+                unrolled<KS>([&](auto ks_c) {
+                    constexpr int ks = decltype(ks_c)::value;
+                    uint32_t a[4];
+                    load_matrices<mt * 16 * D>(k_from[ks], a);
+                    if constexpr (CODE == kCodeE4M3) {
+                        uint32_t x[4], y[4];  // halves 0, 1 and 2, 3 of each word
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) decode4<CODE>(a[i], x[i], y[i]);
+#pragma unroll
+                        for (int nh = 0; nh < NH; ++nh) {
+                            mma_f16<ks == 0>(s[mt][nh], x[0], x[1], x[2], x[3], q[nh][ks][0], q[nh][ks][1]);
+                            mma_f16<false>(s[mt][nh], y[0], y[1], y[2], y[3], q[nh][ks][2], q[nh][ks][3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int nh = 0; nh < NH; ++nh) {
+                            mma_int8<ks == 0>(hi[nh], a, q[nh][ks][0], q[nh][ks][1]);
+                            mma_int8<ks == 0>(lo[nh], a, q[nh][ks][2], q[nh][ks][3]);
+                        }
+                    }
+                });
+                const float2 kv0 = lds_float2<mt * 128>(f0 + first * 8), kv1 = lds_float2<mt * 128>(f1 + first * 8);
+                v_weight[mt][0] = kv0.y;
+                v_weight[mt][1] = kv1.y;
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
+                    if constexpr (CODE == kCodeInt8) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)  // below 2^30 for D = 128
+                            s[mt][nh][e] = static_cast<float>(hi[nh][e] * 256 + lo[nh][e]);
+                    }
+                    s[mt][nh][0] *= kv0.x;
+                    s[mt][nh][1] *= kv0.x;
+                    s[mt][nh][2] *= kv1.x;
+                    s[mt][nh][3] *= kv1.x;
+                }
+            });
+            if (partial) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const bool ok0 = valid(first + mt * 16 + row_g), ok1 = valid(first + mt * 16 + (row_g ^ 1));
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh) {
+                        if (!ok0) s[mt][nh][0] = s[mt][nh][1] = -INFINITY;
+                        if (!ok1) s[mt][nh][2] = s[mt][nh][3] = -INFINITY;
+                    }
+                }
+            }
+
+            // Online softmax.  The running maximum is subtracted before row_scale is applied, so that the largest p
+            // is exactly 1 however large the scores are (fma(s, scale, -max * scale) makes it 2^(rounding of the product)).
+            float sub[NH][2], alpha[NH][2];
+            bool same = unit == 1.0f;
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][nh][h], s[mt][nh][2 + h]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    same = same && !(x > m[nh][h]);
+                    x = fmaxf(m[nh][h], x);
+                    sub[nh][h] = x == -INFINITY ? 0.0f : x;
+                    alpha[nh][h] = m[nh][h];
+                    m[nh][h] = x;
+                }
+            }
+            if (!__all_sync(0xffffffffu, same)) {  // a new maximum or unit: after a row's first tiles rarely
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        alpha[nh][h] = exp2f((alpha[nh][h] - sub[nh][h]) * row_scale[nh][h]);
+                        l[nh][h] *= alpha[nh][h];
+                        alpha[nh][h] *= unit;
+                    }
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        o[nh][i][0] *= alpha[nh][0];
+                        o[nh][i][1] *= alpha[nh][1];
+                        o[nh][i][2] *= alpha[nh][0];
+                        o[nh][i][3] *= alpha[nh][1];
+                    }
+                }
+                unit = 1.0f;
+            }
+
+            unrolled<MT>([&](auto mt_c) {
+                constexpr int mt = decltype(mt_c)::value;
+                const float v0 = v_weight[mt][0], v1 = v_weight[mt][1];
+                uint32_t b[NH][2];
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
+                    const float p0 = exp2f((s[mt][nh][0] - sub[nh][0]) * row_scale[nh][0]);
+                    const float p1 = exp2f((s[mt][nh][1] - sub[nh][1]) * row_scale[nh][1]);
+                    const float p2 = exp2f((s[mt][nh][2] - sub[nh][0]) * row_scale[nh][0]);
+                    const float p3 = exp2f((s[mt][nh][3] - sub[nh][1]) * row_scale[nh][1]);
+                    l[nh][0] += p0 + p2;
+                    l[nh][1] += p1 + p3;
+                    b[nh][0] = transpose8(pack_halves(p0 * v0, p1 * v0));
+                    b[nh][1] = transpose8(pack_halves(p2 * v1, p3 * v1));
+                }
+                // The lane's D/8 bytes of its four tokens; two tokens are interleaved byte by byte, so that one
+                // conversion yields one operand register.  Byte 2 i is row g of output tile i, byte 2 i + 1 row g + 8.
+                uint32_t v[4][D / 32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if constexpr (D == 128) {
+                        const uint4 x = lds128<mt * 16 * D>(v_at[c] + first * D);
+                        v[c][0] = x.x; v[c][1] = x.y; v[c][2] = x.z; v[c][3] = x.w;
+                    } else {
+                        const uint2 x = lds64<mt * 16 * D>(v_at[c] + first * D);
+                        v[c][0] = x.x; v[c][1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    uint32_t a[2][4];
+                    decode4<CODE>(__byte_perm(v[0][i], v[1][i], 0x5140), a[0][0], a[0][1]);
+                    decode4<CODE>(__byte_perm(v[0][i], v[1][i], 0x7362), a[1][0], a[1][1]);
+                    decode4<CODE>(__byte_perm(v[2][i], v[3][i], 0x5140), a[0][2], a[0][3]);
+                    decode4<CODE>(__byte_perm(v[2][i], v[3][i], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh) {
+                        mma_f16<false>(o[nh][2 * i], a[0][0], a[0][1], a[0][2], a[0][3], b[nh][0], b[nh][1]);
+                        mma_f16<false>(o[nh][2 * i + 1], a[1][0], a[1][1], a[1][2], a[1][3], b[nh][0], b[nh][1]);
+                    }
+                }
+            });
+        }
+    }
+
+    // The warp's state into its area: rows of `stride` floats, (o[D], m, l), m in base-2 scores.
+    __device__ __forceinline__ void store(float *area, int stride, int g, int t4)
+    {
+        const float unit = __uint_as_float(static_cast<uint32_t>(v_exp - 15) << 23);  // 2^(v_exp - 142)
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float sum = l[nh][h];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                float *row = area + (nh * 8 + 2 * t4 + h) * stride;
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        row[g * (D / 8) + 2 * i + e] = has_nan ? __uint_as_float(0x7fffffffu) : o[nh][i][2 * e + h] * unit;
+                if (g == 0) {
+                    row[D] = m[nh][h] * row_scale[nh][h];
+                    row[D + 1] = sum;
+                }
+            }
+        }
+    }
+};
+
+}  // namespace
+}  // namespace sa

@@ -260,14 +260,13 @@ class QuantDecodePlan:
     @classmethod
     def build(cls, query: torch.Tensor, cache: QuantCache, *, output: Optional[torch.Tensor] = None,
               splits: Optional[int] = None, validate_metadata: bool = True, record_page_walk: bool = False,
-              return_state: bool = False, kernel: str = "auto", dynamic_schedule: Optional[bool] = None,
+              return_state: bool = False, kernel: str = "auto",
               row_indices: Optional[torch.Tensor] = None) -> "QuantDecodePlan":
         """Validate once and bind a plan.
 
         ``query`` is ``[B, 1, Hq, D]`` in bf16, fp16 or fp32, the output has its shape and dtype; both
         may be pinned host tensors.  ``return_state`` asks for the unnormalised state instead, fp32
-        ``[B, Hq, D + 2]`` (what ``sa_merge_states`` joins).  ``splits``, ``kernel``, ``dynamic_schedule``,
-        ``record_page_walk`` (paged caches) and ``row_indices`` as in :class:`PagedExactDecodePlan` and
+        ``[B, Hq, D + 2]`` (what ``sa_merge_states`` joins).  ``splits``, ``kernel``, ``record_page_walk`` (paged caches) and ``row_indices`` as in :class:`PagedExactDecodePlan` and
         :class:`ExactDecodePlan`; ``validate_metadata`` checks a paged cache's lengths and page ids
         on the host, once.  Rows of no tokens give zeros.
         """
@@ -306,7 +305,7 @@ class QuantDecodePlan:
                 native._ptr(lens), native.SA_INDEX[lens.dtype] if lens is not None else 0, native._ptr(trace),
                 q_heads, q_sb, q_sh, native.SA_DTYPE[query.dtype],
                 native.SA_OUT_STATE if return_state else native.SA_OUT_FINAL, num_ctas,
-                native._kernel_code(kernel, dynamic_schedule))
+                native._kernel_code(kernel, False))
         plan = native.NativePlan(handle, device, (query, cache, output, workspace, trace))
         if row_indices is not None:
             plan.set_rows(row_indices)
