@@ -13,24 +13,24 @@ constexpr int kStreamWarps = SA_STREAM_WARPS;    // each with its own ring of ti
 #define SA_STREAM_STAGES 1
 #endif
 constexpr int kStreamStages = SA_STREAM_STAGES;  // 16 KB K+V tiles in flight per warp
-#ifndef SA_QUANT_TILE
-#define SA_QUANT_TILE 64
+#ifndef SA_QW64
+#define SA_QW64 8
+#define SA_QT64 64
+#define SA_QS64 2
 #endif
-constexpr int kQuantTileTokens = SA_QUANT_TILE;  // 8-bit caches: 8 KB (D64) or 16 KB (D128) of codes a tile
-#ifndef SA_QUANT_STAGES
-#define SA_QUANT_STAGES(D) (128 / (D))
+#ifndef SA_QW128
+#define SA_QW128 8
+#define SA_QT128 64
+#define SA_QS128 1
 #endif
-#ifndef SA_QUANT_WARPS
-#define SA_QUANT_WARPS 8
-#endif
-constexpr int kQuantWarps = SA_QUANT_WARPS;
+__host__ __device__ constexpr int quant_tile_tokens(int head_dim) { return head_dim == 64 ? SA_QT64 : SA_QT128; }  // 8-bit caches: 8 KB (D64) or 16 KB (D128) of codes a tile
 
-constexpr int warps_of(bool quant) { return quant ? kQuantWarps : kStreamWarps; }
+constexpr int warps_of(int head_dim, bool rows16, bool quant) { return !quant ? kStreamWarps : rows16 ? 8 : head_dim == 64 ? SA_QW64 : SA_QW128; }
 
 // Tiles in flight per warp (the state areas of 16 head rows at D128 leave room for fewer).
 constexpr int stages_of(int head_dim, bool rows16, bool quant)
 {
-    if (quant) return SA_QUANT_STAGES(head_dim);
+    if (quant) return rows16 ? 8192 / (quant_tile_tokens(head_dim) * head_dim) : head_dim == 64 ? SA_QS64 : SA_QS128;
     return (head_dim == 128 && rows16 && kStreamStages > 2) ? 2 : kStreamStages;
 }
 

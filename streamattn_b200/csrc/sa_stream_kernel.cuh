@@ -595,7 +595,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                      const __grid_constant__ StreamParams p)
 {
     constexpr bool QUANT = CODE != kCodeNone;
-    constexpr int TILE_N = QUANT ? kQuantTileTokens : kTileBytes / (D * 2);  // tokens per tile
+    constexpr int TILE_N = QUANT ? quant_tile_tokens(D) : kTileBytes / (D * 2);  // tokens per tile
     constexpr int TILE_BYTES = QUANT ? TILE_N * D : kTileBytes;              // one K or one V tile
     constexpr int STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int SCALE_BYTES = QUANT ? TILE_N * 2 : 0;  // (K, V) scale bytes of a tile
@@ -1616,8 +1616,8 @@ cudaError_t launch_dim(const CUtensorMap &mk, const CUtensorMap &mv, const Strea
 {
     constexpr bool kQuant = CODE != kCodeNone;
     if (rows16)
-        return launch_instance<T, D, warps_of(kQuant), stages_of(D, true, kQuant), true, CODE>(mk, mv, sp, ctas, batch, stream);
-    return launch_instance<T, D, warps_of(kQuant), stages_of(D, false, kQuant), false, CODE>(mk, mv, sp, ctas, batch, stream);
+        return launch_instance<T, D, warps_of(D, true, kQuant), stages_of(D, true, kQuant), true, CODE>(mk, mv, sp, ctas, batch, stream);
+    return launch_instance<T, D, warps_of(D, false, kQuant), stages_of(D, false, kQuant), false, CODE>(mk, mv, sp, ctas, batch, stream);
 }
 
 template <int CODE>

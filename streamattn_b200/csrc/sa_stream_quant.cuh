@@ -67,6 +67,11 @@ __device__ __forceinline__ void sts_float4(uint32_t addr, float a, float b, floa
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
+__device__ __forceinline__ void sts_float2(uint32_t addr, float a, float b)
+{
+    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+}
+
 __device__ __forceinline__ void sts128_zero(uint32_t addr)
 {
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
@@ -250,26 +255,29 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
 
         // The scale bytes become floats once a token: K's as it is, V's relative to the unit.  Tokens that are not
         // there get zeros, and so do their V codes: what the buffers hold for them is stale.
-        uint32_t pairs[PER_LANE / 2];
+        constexpr int WORDS = (PER_LANE + 1) / 2;
+        uint32_t pairs[WORDS];
         if constexpr (PER_LANE == 4) {
             const uint2 x = lds64<0>(sb + lane * 8);
             pairs[0] = x.x;
-            pairs[PER_LANE / 2 - 1] = x.y;
-        } else {
+            pairs[WORDS - 1] = x.y;
+        } else if constexpr (PER_LANE == 2) {
             pairs[0] = lds32<0>(sb + lane * 4);
+        } else {
+            pairs[0] = (lds32<0>(sb + (lane >> 1) * 4) >> ((lane & 1) * 16)) & 0xffffu;
         }
         if (partial) {
 #pragma unroll
-            for (int i = 0; i < PER_LANE / 2; ++i) {
+            for (int i = 0; i < WORDS; ++i) {
                 if (!valid(PER_LANE * lane + 2 * i)) pairs[i] &= 0xffff0000u;
-                if (!valid(PER_LANE * lane + 2 * i + 1)) pairs[i] &= 0x0000ffffu;
+                if (PER_LANE > 1 && !valid(PER_LANE * lane + 2 * i + 1)) pairs[i] &= 0x0000ffffu;
             }
             for (int i = lane; i < TILE_N * (D / 16); i += 32)
                 if (!valid(i / (D / 16))) sts128_zero(vb + i * 16);
         }
         uint32_t my_top = 0, nan_bytes = 0;
 #pragma unroll
-        for (int i = 0; i < PER_LANE / 2; ++i) {
+        for (int i = 0; i < WORDS; ++i) {
             const uint32_t nan = __vcmpeq4(pairs[i], 0xffffffffu);
             pairs[i] &= ~nan;
             nan_bytes |= nan;
@@ -284,11 +292,12 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
         v_exp = max(v_exp, top);
         const int off = (142 - v_exp) * (1 << 23);
 #pragma unroll
-        for (int i = 0; i < PER_LANE / 2; ++i) {
+        for (int i = 0; i < WORDS; ++i) {
             const float k0 = __uint_as_float((pairs[i] << 23) & 0x7f800000u), k1 = __uint_as_float((pairs[i] << 7) & 0x7f800000u);
             const float v0 = __int_as_float(max(static_cast<int>((pairs[i] << 15) & 0x7f800000u) + off, 0));
             const float v1 = __int_as_float(max(static_cast<int>((pairs[i] >> 1) & 0x7f800000u) + off, 0));
-            sts_float4(fb + (PER_LANE * lane + 2 * i) * 8, k0, v0, k1, v1);
+            if constexpr (PER_LANE > 1) sts_float4(fb + (PER_LANE * lane + 2 * i) * 8, k0, v0, k1, v1);
+            else sts_float2(fb + lane * 8, k0, v0);
         }
         __syncwarp();
         float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);
