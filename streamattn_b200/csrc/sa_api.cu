@@ -572,13 +572,21 @@ int fill_quant(sa_plan *plan, const void *q, const sa_quant_cache_t *cache, void
     return finish_plan(plan, workspace, workspace_bytes, c.capacity, kernel_choice);
 }
 
-// Whether rows of `stride`-spaced elements of `size` bytes can be moved in 16-byte pieces.
-bool wide(const void *p, std::initializer_list<int64_t> strides, int size, int align)
+// Whether rows of elements of `size` bytes, spaced by sb (batch rows) and `strides` (tokens, heads, pages), can be
+// moved in pieces of `align` bytes at offsets that are products of 32-bit numbers.
+bool wide(const void *p, int64_t sb, std::initializer_list<int64_t> strides, int size, int align)
 {
-    if (reinterpret_cast<uintptr_t>(p) % align) return false;
+    if (reinterpret_cast<uintptr_t>(p) % align || sb * size % align) return false;
     for (int64_t s : strides)
-        if (s * size % align) return false;
+        if (s * size % align || s >= (1ll << 31) || s < 0) return false;
     return true;
+}
+
+bool wide_cache(const QuantCache &c)
+{
+    const int64_t page = c.page_table != nullptr ? c.so : 0;  // of a contiguous cache `so` is the batch row's stride
+    return c.head_dim % 16 == 0 && wide(c.key, c.so, {page, c.sn, c.sh}, 1, 8) && wide(c.value, 0, {}, 1, 8) &&
+           c.scale_sh < (1ll << 31) && c.num_pages < (1ll << 31);
 }
 
 }  // namespace
@@ -1285,12 +1293,12 @@ int sa_quantize_kv(const sa_quant_cache_t *cache, const void *k_new, const void 
     a.heads_fastest = new_stride_h <= new_stride_t;
     const int size = dtype == SA_DTYPE_F32 ? 4 : 2;
     const QuantCache &c = a.cache;
-    bool vector = c.head_dim % 8 == 0 && wide(k_new, {new_stride_b, new_stride_t, new_stride_h}, size, 16) &&
-                  wide(v_new, {}, size, 16) && wide(c.key, {c.so, c.sn, c.sh}, 1, 8) && wide(c.value, {}, 1, 8);
-    if (cos) vector = vector && c.head_dim % 16 == 0 && wide(cos, {rope_stride_b, rope_stride_t}, size, 16) && wide(sin, {}, size, 16);
+    bool vector = wide_cache(c) && wide(k_new, new_stride_b, {new_stride_t, new_stride_h}, size, 16) && wide(v_new, 0, {}, size, 16);
+    if (cos)
+        vector = vector && wide(cos, rope_stride_b, {rope_stride_t}, size, 16) && wide(sin, 0, {}, size, 16);
     if (q_in)
-        vector = vector && wide(q_in, {q_in_stride_b, q_in_stride_t, q_in_stride_h}, size, 16) &&
-                 wide(q_out, {q_out_stride_b, q_out_stride_t, q_out_stride_h}, size, 16);
+        vector = vector && wide(q_in, q_in_stride_b, {q_in_stride_t, q_in_stride_h}, size, 16) &&
+                 wide(q_out, q_out_stride_b, {q_out_stride_t, q_out_stride_h}, size, 16);
     const cudaError_t err = launch_quantize(a, cache->code, dtype, vector, static_cast<cudaStream_t>(stream));
     if (err != cudaSuccess) return fail_cuda(err, "kernel launch failed");
     return SA_OK;
@@ -1324,8 +1332,7 @@ int sa_dequantize_kv(const sa_quant_cache_t *cache, void *k_out, void *v_out, in
     a.heads_fastest = a.cache.sh <= a.cache.sn;
     const int size = dtype == SA_DTYPE_F32 ? 4 : 2;
     const QuantCache &c = a.cache;
-    const bool vector = c.head_dim % 8 == 0 && wide(k_out, {out_stride_b, out_stride_t, out_stride_h}, size, 16) &&
-                        wide(v_out, {}, size, 16) && wide(c.key, {c.so, c.sn, c.sh}, 1, 8) && wide(c.value, {}, 1, 8);
+    const bool vector = wide_cache(c) && wide(k_out, out_stride_b, {out_stride_t, out_stride_h}, size, 16) && wide(v_out, 0, {}, size, 16);
     const cudaError_t err = launch_dequantize(a, cache->code, dtype, vector, static_cast<cudaStream_t>(stream));
     if (err != cudaSuccess) return fail_cuda(err, "kernel launch failed");
     return SA_OK;

@@ -131,6 +131,20 @@ __device__ __forceinline__ bool locate_token(const QuantCache &c, int b, int pos
     return true;
 }
 
+// n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31+s) / d), which fits 32 bits,
+// floor(n m / 2^(31+s)) = floor(n / d) because m d exceeds 2^(31+s) by less than d <= 2^s.
+struct FastDiv {
+    unsigned d, magic;
+    int shift;  // s - 1; -1: d == 1
+    FastDiv() = default;
+    explicit FastDiv(unsigned divisor) : d(divisor), magic(0), shift(-1)
+    {
+        while (shift < 30 && (1u << (shift + 1)) < d) ++shift;
+        if (shift >= 0) magic = static_cast<unsigned>(((1ull << (32 + shift)) + d - 1) / d);
+    }
+    __device__ __forceinline__ unsigned divide(unsigned n) const { return shift < 0 ? n : __umulhi(n, magic) >> shift; }
+};
+
 struct QuantizeParams {
     QuantCache cache;
     const void *k_new;
@@ -152,6 +166,7 @@ struct QuantizeParams {
     int *status;
     int heads_fastest;                // order in which a row's (token, head) units are taken
     int kv_blocks;                    // CTAs of one batch row that write K/V; the others move the query
+    FastDiv kv_div, q_div;            // by the index of a unit that varies fastest
 };
 
 struct DequantizeParams {
@@ -166,9 +181,10 @@ struct DequantizeParams {
     int counts_i64;
     int *status;
     int heads_fastest;
+    FastDiv div;
 };
 
-// `vector`: head_dim, strides and addresses allow 8-element accesses.
+// `vector`: head_dim is a multiple of 16, addresses allow 8-element accesses, and every stride but the batch row's fits 32 bits.
 cudaError_t launch_quantize(QuantizeParams p, int code, int dtype, bool vector, cudaStream_t stream);
 cudaError_t launch_dequantize(DequantizeParams p, int code, int dtype, bool vector, cudaStream_t stream);
 

@@ -2,18 +2,20 @@
 // cache, and read rows back.  The format is described in sa_quant.cuh.
 //
 // Both are one pass over the data and bound by memory: D * (element + 1) + 1 bytes a row.  A unit is
-// the K and the V row of one (token, head); ceil(D / 8) lanes (rounded up to a power of two) share
-// it, 8 elements each, so 16-bit rows move in 16-byte and codes in 8-byte pieces, the maximum of a
-// row is a few shuffles, and the two scale bytes of a token leave in one 2-byte store.  Every
-// thread requests all of its kUnits units before it looks at the first.  Rows that do not allow
-// such accesses (odd sizes, odd strides) take one warp a unit with single-element accesses.
+// the K and the V row of one (token, head); D / 16 lanes (rounded up to a power of two) share it,
+// 8 elements of either half of the row each, so 16-bit rows move in 16-byte and codes in 8-byte
+// pieces, the maximum of a row is a few shuffles, and the two scale bytes of a token leave in one
+// 2-byte store.  A thread requests all that it reads before it writes anything.  Rows that do not allow
+// such accesses (D no multiple of 16, odd strides) take one warp a unit with single-element accesses.
+#include <algorithm>
+
 #include "sa_quant.cuh"
 
 namespace sa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;        // units a lane group has in flight
+constexpr int kScalarUnits = 2;  // units a warp of the scalar kernels takes
 constexpr int kMaxLaneElems = 8; // scalar form: elements of a row a lane holds (head_dim <= 256)
 
 __device__ __forceinline__ void wait_for_stream()
@@ -28,6 +30,16 @@ __device__ __forceinline__ void wait_for_stream()
 template <typename T> struct Eight;
 template <> struct Eight<float> {
     float4 a, b;
+    // Bits of the largest magnitude (a NaN is larger than an infinity, an infinity larger than a number).
+    __device__ __forceinline__ uint32_t top() const
+    {
+        float x[8];
+        get(x);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+        return m;
+    }
     __device__ __forceinline__ void load(const float *p)
     {
         a = reinterpret_cast<const float4 *>(p)[0];
@@ -46,6 +58,12 @@ template <> struct Eight<float> {
 };
 template <typename T> struct Eight {
     uint4 a;
+    __device__ __forceinline__ uint32_t top() const  // two 16-bit patterns at a time: their order is that of the magnitudes
+    {
+        const uint32_t m = __vmaxu2(__vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu), __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu));
+        const uint16_t pattern = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+        return __float_as_uint(Elem<T>::to_float(*reinterpret_cast<const T *>(&pattern)));
+    }
     __device__ __forceinline__ void load(const T *p) { a = *reinterpret_cast<const uint4 *>(p); }
     __device__ __forceinline__ void get(float (&x)[8]) const
     {
@@ -99,160 +117,183 @@ __device__ __forceinline__ void report(int *status, int bits)
     if (status != nullptr) atomicOr(status, bits);
 }
 
-// Writes position + count of row b where every page of the range exists (whole CTA; `bad` is the
-// CTA's own shared flag).
-__device__ __forceinline__ void store_length(const QuantizeParams &p, int b, const RowPlace &r, int *bad)
+__device__ __forceinline__ void put_length(const QuantizeParams &p, int b, const RowPlace &r)
 {
-    if (threadIdx.x == 0) *bad = r.ok ? 0 : 1;
-    __syncthreads();  // and: every thread of the CTA has read its position
-    if (r.ok && p.cache.page_table != nullptr && r.count > 0) {
-        const int first = r.start / p.cache.page_size, last = (r.start + r.count - 1) / p.cache.page_size;
-        for (int lp = first + threadIdx.x; lp <= last; lp += blockDim.x) {
-            const int64_t page = load_index(p.cache.page_table, p.cache.table_i64, static_cast<int64_t>(b) * p.cache.max_pages + lp);
-            if (page < 0 || page >= p.cache.num_pages) *bad = 1;
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0 && *bad == 0) {
-        if (p.pos_i64) static_cast<int64_t *>(p.lens_out)[b] = static_cast<int64_t>(r.start) + r.count;
-        else static_cast<int32_t *>(p.lens_out)[b] = r.start + r.count;
-    }
+    if (p.pos_i64) static_cast<int64_t *>(p.lens_out)[b] = static_cast<int64_t>(r.start) + r.count;
+    else static_cast<int32_t *>(p.lens_out)[b] = r.start + r.count;
 }
 
-// unit -> (token, head)
-__device__ __forceinline__ void unit_of(unsigned unit, unsigned heads, unsigned tokens, int heads_fastest, int &t, int &h)
+// unit -> (token, head), the inner one of the two varying fastest.
+__device__ __forceinline__ void unit_of(unsigned unit, const FastDiv &inner, int heads_fastest, int &t, int &h)
 {
-    const unsigned inner = heads_fastest ? heads : tokens;
-    const unsigned outer_index = unit / inner, inner_index = unit - outer_index * inner;
+    const unsigned outer_index = inner.divide(unit), inner_index = unit - outer_index * inner.d;
     t = static_cast<int>(heads_fastest ? outer_index : inner_index);
     h = static_cast<int>(heads_fastest ? inner_index : outer_index);
 }
 
-// One K or V row of a unit, eight elements a lane: scale byte from the maximum over the `lanes`
-// lanes that share the row, then the codes.
-template <int CODE> __device__ __forceinline__ int quantize_eight(const float (&x)[8], int lanes, uint2 &codes)
+// Offset i * stride for strides that fit 32 bits (the vector kernels; the host checks): one instruction.
+__device__ __forceinline__ int64_t at(int i, int64_t stride) { return static_cast<int64_t>(i) * static_cast<int>(stride); }
+
+// Token `pos` of row b for the vector kernels: code and pair offsets of head 0; false where its page id names no page.
+__device__ __forceinline__ bool place_token(const QuantCache &c, int b, int pos, int64_t &code_off, int64_t &pair_off)
 {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);  // a NaN is the largest
-    for (int o = lanes >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const int e = scale_byte<CODE>(amax);
-    const float inv = inverse_scale(e);
-    codes.x = encode4<CODE>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    codes.y = encode4<CODE>(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-    if (e == kNanScaleByte) codes = make_uint2(0u, 0u);
-    return e;
+    if (c.page_table == nullptr) {
+        code_off = b * c.so + at(pos, c.sn);
+        pair_off = b * c.scale_so + pos;
+        return true;
+    }
+    const int lp = c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page_size;
+    const int slot = pos - lp * c.page_size;
+    const int64_t page = load_index(c.page_table, c.table_i64, static_cast<int64_t>(b) * c.max_pages + lp);
+    if (page < 0 || page >= c.num_pages) return false;
+    code_off = at(static_cast<int>(page), c.so) + at(slot, c.sn);
+    pair_off = at(static_cast<int>(page), c.scale_so) + slot;
+    return true;
 }
 
-template <typename T, int CODE>
-__global__ void __launch_bounds__(kThreads) quantize_vector_kernel(const __grid_constant__ QuantizeParams p, int lanes)
+// Codes of eight values of a row with scale byte e.
+template <int CODE> __device__ __forceinline__ uint2 encode8(const float (&x)[8], int e)
 {
-    __shared__ int bad;
+    const float inv = inverse_scale(e);
+    uint2 codes;
+    if constexpr (CODE == kCodeE4M3) {
+        codes.x = encode4<CODE>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        codes.y = encode4<CODE>(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+    } else {
+        // x * inv is exact and at most 127 in magnitude; added to 1.5 * 2^23 it is rounded to an integer, halves to
+        // even, whose two's complement is the sum's lowest byte.
+        uint32_t y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __float_as_uint(__fmaf_rn(x[i], inv, 12582912.0f));
+        codes.x = __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
+        codes.y = __byte_perm(__byte_perm(y[4], y[5], 0x0040), __byte_perm(y[6], y[7], 0x0040), 0x5410);
+    }
+    return e == kNanScaleByte ? make_uint2(0u, 0u) : codes;
+}
+
+// The two pieces of a row a lane holds: elements d .. d + 7 of each half of the row, so that the lanes of a row read
+// consecutive pieces and every element finds the one it is rotated with in the same lane.
+template <typename T> struct Halves {
+    Eight<T> lo, hi;
+    __device__ __forceinline__ void load(const T *row, int half)
+    {
+        lo.load(row);
+        hi.load(row + half);
+    }
+    __device__ __forceinline__ void get(float (&x)[8], float (&y)[8]) const
+    {
+        lo.get(x);
+        hi.get(y);
+    }
+    __device__ __forceinline__ void turned(const Halves &cos, const Halves &sin, float (&x)[8], float (&y)[8]) const
+    {
+        float a[8], b[8], c[8], s[8];
+        get(a, b);
+        cos.lo.get(c);
+        sin.lo.get(s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = rotate(a[i], b[i], true, c[i], s[i]);
+        cos.hi.get(c);
+        sin.hi.get(s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = rotate(b[i], a[i], false, c[i], s[i]);
+    }
+};
+
+template <typename T, int CODE, bool ROPE>
+__global__ void __launch_bounds__(kThreads) quantize_vector_kernel(const __grid_constant__ QuantizeParams p, int lane_shift)
+{
     wait_for_stream();
     const int b = blockIdx.y;
-    const int dim = p.cache.head_dim, half = dim >> 1;
-    const int groups = kThreads / lanes;             // units the CTA handles at a time
-    const int group = threadIdx.x / lanes;
-    const int d = (threadIdx.x - group * lanes) * 8;
-    const bool in_row = d < dim;
-    const bool rope = p.cos != nullptr;
-    const T *cos_b = static_cast<const T *>(p.cos) + b * p.rope_sb;
-    const T *sin_b = static_cast<const T *>(p.sin) + b * p.rope_sb;
+    const int half = p.cache.head_dim >> 1;
+    const int lanes = 1 << lane_shift;
+    const int d = (threadIdx.x & (lanes - 1)) * 8;
+    const bool in_row = d < half;
+    const bool is_query = static_cast<int>(blockIdx.x) >= p.kv_blocks;
+    const unsigned first = (blockIdx.x - (is_query ? p.kv_blocks : 0)) * (kThreads >> lane_shift);  // the CTA's first unit
+    const unsigned unit = first + (threadIdx.x >> lane_shift);
+    const FastDiv &div = is_query ? p.q_div : p.kv_div;
+    int t, h;
+    unit_of(unit, div, p.heads_fastest, t, h);
+    const T *cos = static_cast<const T *>(p.cos) + b * p.rope_sb + at(t, p.rope_st) + d;
+    const T *sin = static_cast<const T *>(p.sin) + b * p.rope_sb + at(t, p.rope_st) + d;
+    Halves<T> c, s;
+    float x[8], y[8];
 
-    if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {  // query rows
+    if (is_query) {
         const int count = clipped_count(p.counts, p.counts_i64, b, p.tokens);
-        const unsigned total = static_cast<unsigned>(p.tokens) * p.q_heads;
-        const unsigned first = (blockIdx.x - p.kv_blocks) * groups * kUnits + group;
-        for (int u = 0; u < kUnits; ++u) {
-            const unsigned unit = first + u * groups;
-            int t, h;
-            unit_of(unit, p.q_heads, p.tokens, p.heads_fastest, t, h);
-            if (unit >= total || t >= count || !in_row) continue;
-            const T *src = static_cast<const T *>(p.q_in) + b * p.qi_sb + t * p.qi_st + h * p.qi_sh;
-            Eight<T> raw;
-            raw.load(src + d);
-            float x[8];
-            raw.get(x);
-            if (rope) {
-                float y[8], c[8], s[8];
-                raw.load(src + (d < half ? d + half : d - half));
-                raw.get(y);
-                raw.load(cos_b + t * p.rope_st + d);
-                raw.get(c);
-                raw.load(sin_b + t * p.rope_st + d);
-                raw.get(s);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = rotate(x[i], y[i], d < half, c[i], s[i]);
-            }
-            Eight<T>::store(static_cast<T *>(p.q_out) + b * p.qo_sb + t * p.qo_st + h * p.qo_sh + d, x);
+        if (unit >= static_cast<unsigned>(p.tokens) * p.q_heads || t >= count || !in_row) return;
+        Halves<T> q;
+        q.load(static_cast<const T *>(p.q_in) + b * p.qi_sb + at(t, p.qi_st) + at(h, p.qi_sh) + d, half);
+        if (ROPE) {
+            c.load(cos, half);
+            s.load(sin, half);
+            q.turned(c, s, x, y);
+        } else {
+            q.get(x, y);
         }
+        T *out = static_cast<T *>(p.q_out) + b * p.qo_sb + at(t, p.qo_st) + at(h, p.qo_sh) + d;
+        Eight<T>::store(out, x);
+        Eight<T>::store(out + half, y);
         return;
     }
 
     const RowPlace place = row_place(p, b);
+    const bool alone = p.kv_blocks == 1;  // the only CTA that reads this row's position: it may also replace it
     if (!place.ok && threadIdx.x == 0) report(p.status, SA_DEV_BAD_POSITION);
-    const unsigned total = static_cast<unsigned>(p.tokens) * p.cache.kv_heads;   // < 2^30: the host checks
-    const unsigned first = blockIdx.x * groups * kUnits + group;
-    Eight<T> k[kUnits], v[kUnits], partner[kUnits];
-    int t[kUnits], h[kUnits];
-    bool active[kUnits];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        const unsigned unit = first + u * groups;
-        unit_of(unit, p.cache.kv_heads, p.tokens, p.heads_fastest, t[u], h[u]);
-        active[u] = place.ok && unit < total && t[u] < place.count;
-        if (active[u] && in_row) {
-            const int64_t src = b * p.new_sb + t[u] * p.new_st + h[u] * p.new_sh;
-            k[u].load(static_cast<const T *>(p.k_new) + src + d);
-            v[u].load(static_cast<const T *>(p.v_new) + src + d);
-            if (rope) partner[u].load(static_cast<const T *>(p.k_new) + src + (d < half ? d + half : d - half));
+    if (!alone && p.heads_fastest && div.divide(first) >= static_cast<unsigned>(place.count)) return;  // padding
+    // Everything that is read - rows, angles, page id - is requested before anything is written.
+    const bool mine = place.ok && unit < static_cast<unsigned>(p.tokens) * p.cache.kv_heads && t < place.count && in_row;
+    Halves<T> k, v;
+    int64_t code_off = 0, pair_off = 0;
+    bool there = true;  // the token's page
+    uint32_t e = 0;     // scale bytes of K and V, side by side
+    if (mine) {
+        const int64_t src = b * p.new_sb + at(t, p.new_st) + at(h, p.new_sh) + d;
+        k.load(static_cast<const T *>(p.k_new) + src, half);
+        v.load(static_cast<const T *>(p.v_new) + src, half);
+        if (ROPE) {
+            c.load(cos, half);
+            s.load(sin, half);
         }
+        there = place_token(p.cache, b, place.start + t, code_off, pair_off);
+        uint32_t k_top = 0;
+        if (ROPE) {
+            k.turned(c, s, x, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                k_top = max(k_top, max(__float_as_uint(x[i]) & 0x7fffffffu, __float_as_uint(y[i]) & 0x7fffffffu));
+        } else {
+            k.get(x, y);
+            k_top = max(k.lo.top(), k.hi.top());
+        }
+        e = scale_byte<CODE>(k_top) | (scale_byte<CODE>(max(v.lo.top(), v.hi.top())) << 16);
     }
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        float x[8], y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.0f;   // lanes without a part of the row
-        if (active[u] && in_row) {
-            k[u].get(x);
-            v[u].get(y);
-            if (rope) {
-                float other[8], c[8], s[8];
-                Eight<T> raw;
-                partner[u].get(other);
-                raw.load(cos_b + t[u] * p.rope_st + d);
-                raw.get(c);
-                raw.load(sin_b + t[u] * p.rope_st + d);
-                raw.get(s);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = rotate(x[i], other[i], d < half, c[i], s[i]);
-            }
-        }
-        uint2 k_codes, v_codes;
-        const int ek = quantize_eight<CODE>(x, lanes, k_codes);   // all lanes: shuffles inside
-        const int ev = quantize_eight<CODE>(y, lanes, v_codes);
-        if (!active[u] || !in_row) continue;
-        int64_t code_off, pair_off;
-        if (!locate_token(p.cache, b, place.start + t[u], code_off, pair_off)) {
-            if (d == 0) report(p.status, SA_DEV_BAD_PAGE);
-            continue;
-        }
-        code_off += h[u] * p.cache.sh + d;
-        *reinterpret_cast<uint2 *>(p.cache.key + code_off) = k_codes;
-        *reinterpret_cast<uint2 *>(p.cache.value + code_off) = v_codes;
+    // The scale byte grows with the largest magnitude: a row's byte is the largest of its lanes' bytes.
+    for (int o = lanes >> 1; o > 0; o >>= 1) e = __vmaxu2(e, __shfl_xor_sync(0xffffffffu, e, o));
+    if (mine && there) {
+        const int ek = e & 0xffffu, ev = e >> 16;
+        uint8_t *key = p.cache.key + code_off + at(h, p.cache.sh) + d, *value = p.cache.value + code_off + at(h, p.cache.sh) + d;
+        *reinterpret_cast<uint2 *>(key) = encode8<CODE>(x, ek);
+        *reinterpret_cast<uint2 *>(key + half) = encode8<CODE>(y, ek);
+        v.get(x, y);
+        *reinterpret_cast<uint2 *>(value) = encode8<CODE>(x, ev);
+        *reinterpret_cast<uint2 *>(value + half) = encode8<CODE>(y, ev);
         if (d == 0)
-            reinterpret_cast<uint16_t *>(p.cache.scales)[pair_off + h[u] * p.cache.scale_sh] =
-                static_cast<uint16_t>(ek | (ev << 8));
+            reinterpret_cast<uint16_t *>(p.cache.scales)[pair_off + at(h, p.cache.scale_sh)] = static_cast<uint16_t>(ek | (ev << 8));
+    } else if (mine && d == 0) {
+        report(p.status, SA_DEV_BAD_PAGE);
     }
-    // The only CTA that reads this row's position may also replace it.
-    if (p.lens_out != nullptr && p.kv_blocks == 1) store_length(p, b, place, &bad);
+    if (alone && p.lens_out != nullptr) {
+        const bool bad = __syncthreads_or(!there) || !place.ok;  // and: every thread has read its position
+        if (threadIdx.x == 0 && !bad) put_length(p, b, place);
+    }
 }
 
 // One warp a unit, single-element accesses: any head_dim up to 256, any stride.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(kThreads) quantize_scalar_kernel(const __grid_constant__ QuantizeParams p)
 {
-    __shared__ int bad;
     wait_for_stream();
     const int b = blockIdx.y;
     const int dim = p.cache.head_dim, half = dim >> 1;
@@ -264,13 +305,14 @@ __global__ void __launch_bounds__(kThreads) quantize_scalar_kernel(const __grid_
     const RowPlace place = is_query ? RowPlace{0, clipped_count(p.counts, p.counts_i64, b, p.tokens), true} : row_place(p, b);
     const int heads = is_query ? p.q_heads : p.cache.kv_heads;
     const unsigned total = static_cast<unsigned>(p.tokens) * heads;
-    const unsigned first = (blockIdx.x - (is_query ? p.kv_blocks : 0)) * kWarps * kUnits + warp;
+    const unsigned first = (blockIdx.x - (is_query ? p.kv_blocks : 0)) * kWarps * kScalarUnits + warp;
     if (!is_query && !place.ok && threadIdx.x == 0) report(p.status, SA_DEV_BAD_POSITION);
+    bool bad = !place.ok;
 
-    for (int u = 0; u < kUnits; ++u) {
+    for (int u = 0; u < kScalarUnits; ++u) {
         const unsigned unit = first + u * kWarps;
         int t, h;
-        unit_of(unit, heads, p.tokens, p.heads_fastest, t, h);
+        unit_of(unit, is_query ? p.q_div : p.kv_div, p.heads_fastest, t, h);
         if (unit >= total || t >= place.count) continue;        // warp-uniform, like everything down to the stores
         const T *cos_row = static_cast<const T *>(p.cos) + b * p.rope_sb + t * p.rope_st;
         const T *sin_row = static_cast<const T *>(p.sin) + b * p.rope_sb + t * p.rope_st;
@@ -290,6 +332,7 @@ __global__ void __launch_bounds__(kThreads) quantize_scalar_kernel(const __grid_
         int64_t code_off, pair_off;
         if (!locate_token(p.cache, b, place.start + t, code_off, pair_off)) {
             if (lane == 0) report(p.status, SA_DEV_BAD_PAGE);
+            bad = true;
             continue;
         }
         const int64_t src = b * p.new_sb + t * p.new_st + h * p.new_sh;
@@ -320,91 +363,122 @@ __global__ void __launch_bounds__(kThreads) quantize_scalar_kernel(const __grid_
             reinterpret_cast<uint16_t *>(p.cache.scales)[pair_off + h * p.cache.scale_sh] =
                 static_cast<uint16_t>(e[0] | (e[1] << 8));
     }
-    if (!is_query && p.lens_out != nullptr && p.kv_blocks == 1) store_length(p, b, place, &bad);
+    if (!is_query && p.lens_out != nullptr && p.kv_blocks == 1) {  // as above
+        bad = __syncthreads_or(bad);
+        if (threadIdx.x == 0 && !bad) put_length(p, b, place);
+    }
 }
 
-// Rows whose tokens were written by several CTAs: the lengths, after all of them.
+// Rows whose tokens were written by several CTAs: the lengths, after all of them, where every page of the range exists.
 __global__ void __launch_bounds__(128) quantize_lengths_kernel(const __grid_constant__ QuantizeParams p)
 {
-    __shared__ int bad;
     wait_for_stream();
-    store_length(p, blockIdx.x, row_place(p, blockIdx.x), &bad);
+    const int b = blockIdx.x;
+    const RowPlace r = row_place(p, b);
+    bool bad = !r.ok;
+    if (r.ok && p.cache.page_table != nullptr && r.count > 0) {
+        const int first = r.start / p.cache.page_size, last = (r.start + r.count - 1) / p.cache.page_size;
+        for (int lp = first + threadIdx.x; lp <= last; lp += blockDim.x) {
+            const int64_t page = load_index(p.cache.page_table, p.cache.table_i64, static_cast<int64_t>(b) * p.cache.max_pages + lp);
+            bad = bad || page < 0 || page >= p.cache.num_pages;
+        }
+    }
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0 && !bad) put_length(p, b, r);
 }
 
-template <typename T, int CODE, bool VECTOR>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const __grid_constant__ DequantizeParams p, int lanes)
+template <typename T, int CODE>
+__global__ void __launch_bounds__(kThreads) dequantize_vector_kernel(const __grid_constant__ DequantizeParams p, int lane_shift)
 {
     wait_for_stream();
     const int b = blockIdx.y;
-    const int dim = p.cache.head_dim;
-    const int groups = kThreads / lanes;
-    const int group = threadIdx.x / lanes;
-    const int d = (threadIdx.x - group * lanes) * (VECTOR ? 8 : 1);
-    const int64_t start = p.starts == nullptr ? 0 : load_index(p.starts, p.starts_i64, b);
+    const int half = p.cache.head_dim >> 1;
+    const int d = (threadIdx.x & ((1 << lane_shift) - 1)) * 8;
+    const unsigned unit = blockIdx.x * (kThreads >> lane_shift) + (threadIdx.x >> lane_shift);
+    int t, h;
+    unit_of(unit, p.div, p.heads_fastest, t, h);
+    const int64_t pos = (p.starts == nullptr ? 0 : load_index(p.starts, p.starts_i64, b)) + t;
     const int count = clipped_count(p.counts, p.counts_i64, b, p.tokens);
-    const unsigned total = static_cast<unsigned>(p.tokens) * p.cache.kv_heads;   // < 2^30: the host checks
-    const unsigned first = blockIdx.x * groups * kUnits + group;
-    uint2 k[kUnits], v[kUnits];
-    uint32_t pair[kUnits];
-    int64_t from[kUnits], to[kUnits];   // code offset of the unit's row (-1: nothing to do), output offset
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        const unsigned unit = first + u * groups;
-        int t, h;
-        unit_of(unit, p.cache.kv_heads, p.tokens, p.heads_fastest, t, h);
-        from[u] = -1;
-        if (unit >= total || t >= count || d >= dim) continue;
-        const int64_t pos = start + t;
-        int64_t code_off, pair_off;
-        if (pos < 0 || pos >= p.cache.capacity) {
-            if (d == 0) report(p.status, SA_DEV_BAD_POSITION);
-        } else if (!locate_token(p.cache, b, static_cast<int>(pos), code_off, pair_off)) {
-            if (d == 0) report(p.status, SA_DEV_BAD_PAGE);
-        } else {
-            from[u] = code_off + h * p.cache.sh;
-            to[u] = b * p.out_sb + t * p.out_st + h * p.out_sh;
-            pair[u] = reinterpret_cast<const uint16_t *>(p.cache.scales)[pair_off + h * p.cache.scale_sh];
-            if (VECTOR) {
-                k[u] = *reinterpret_cast<const uint2 *>(p.cache.key + from[u] + d);
-                v[u] = *reinterpret_cast<const uint2 *>(p.cache.value + from[u] + d);
-            }
-        }
+    if (unit >= static_cast<unsigned>(p.tokens) * p.cache.kv_heads || t >= count || d >= half) return;
+    int64_t code_off, pair_off;
+    int bad = 0;
+    if (pos < 0 || pos >= p.cache.capacity) bad = SA_DEV_BAD_POSITION;
+    else if (!place_token(p.cache, b, static_cast<int>(pos), code_off, pair_off)) bad = SA_DEV_BAD_PAGE;
+    if (bad != 0) {
+        if (d == 0) report(p.status, bad);
+        return;
     }
+    code_off += at(h, p.cache.sh) + d;
+    const uint32_t pair = reinterpret_cast<const uint16_t *>(p.cache.scales)[pair_off + at(h, p.cache.scale_sh)];
+    uint2 codes[2][2];
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        if (from[u] < 0) continue;
-        const float sk = scale_value(pair[u] & 0xffu), sv = scale_value(pair[u] >> 8);
-        T *k_row = static_cast<T *>(p.k_out) + to[u], *v_row = static_cast<T *>(p.v_out) + to[u];
-        if (VECTOR) {
-            auto put = [&](uint2 codes, float scale, T *row) {
-                float x[8];
+    for (int i = 0; i < 2; ++i) {
+        codes[0][i] = *reinterpret_cast<const uint2 *>(p.cache.key + code_off + i * half);
+        codes[1][i] = *reinterpret_cast<const uint2 *>(p.cache.value + code_off + i * half);
+    }
+    const int64_t to = b * p.out_sb + at(t, p.out_st) + at(h, p.out_sh) + d;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t lo, hi;
-                    decode4<CODE>(i ? codes.y : codes.x, lo, hi);
-                    const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&lo));
-                    const float2 c = __half22float2(*reinterpret_cast<__half2 *>(&hi));
-                    x[4 * i] = a.x * scale; x[4 * i + 1] = a.y * scale;
-                    x[4 * i + 2] = c.x * scale; x[4 * i + 3] = c.y * scale;
-                }
-                Eight<T>::store(row + d, x);
-            };
-            put(k[u], sk, k_row);
-            put(v[u], sv, v_row);
-        } else {
-            for (int i = d; i < dim; i += lanes) {
-                k_row[i] = Elem<T>::from_float(decode1<CODE>(p.cache.key[from[u] + i]) * sk);
-                v_row[i] = Elem<T>::from_float(decode1<CODE>(p.cache.value[from[u] + i]) * sv);
+    for (int which = 0; which < 2; ++which) {
+        const float scale = scale_value(which ? pair >> 8 : pair & 0xffu);
+        T *row = static_cast<T *>(which ? p.v_out : p.k_out) + to;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float x[8];
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                uint32_t lo, hi;
+                decode4<CODE>(w ? codes[which][i].y : codes[which][i].x, lo, hi);
+                const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&lo));
+                const float2 c = __half22float2(*reinterpret_cast<__half2 *>(&hi));
+                x[4 * w] = a.x * scale; x[4 * w + 1] = a.y * scale;
+                x[4 * w + 2] = c.x * scale; x[4 * w + 3] = c.y * scale;
             }
+            Eight<T>::store(row + i * half, x);
         }
     }
 }
 
-int lanes_per_row(int dim)
+// One warp a unit, single-element accesses.
+template <typename T, int CODE>
+__global__ void __launch_bounds__(kThreads) dequantize_scalar_kernel(const __grid_constant__ DequantizeParams p)
 {
-    int lanes = 1;
-    while (lanes * 8 < dim) lanes <<= 1;
-    return lanes;
+    wait_for_stream();
+    const int b = blockIdx.y;
+    const int lane = threadIdx.x & 31;
+    constexpr int kWarps = kThreads / 32;
+    const int64_t start = p.starts == nullptr ? 0 : load_index(p.starts, p.starts_i64, b);
+    const int count = clipped_count(p.counts, p.counts_i64, b, p.tokens);
+    const unsigned total = static_cast<unsigned>(p.tokens) * p.cache.kv_heads;
+    for (int u = 0; u < kScalarUnits; ++u) {
+        const unsigned unit = (blockIdx.x * kScalarUnits + u) * kWarps + (threadIdx.x >> 5);
+        int t, h;
+        unit_of(unit, p.div, p.heads_fastest, t, h);
+        if (unit >= total || t >= count) continue;
+        const int64_t pos = start + t;
+        int64_t code_off, pair_off;
+        int bad = 0;
+        if (pos < 0 || pos >= p.cache.capacity) bad = SA_DEV_BAD_POSITION;
+        else if (!locate_token(p.cache, b, static_cast<int>(pos), code_off, pair_off)) bad = SA_DEV_BAD_PAGE;
+        if (bad != 0) {
+            if (lane == 0) report(p.status, bad);
+            continue;
+        }
+        code_off += h * p.cache.sh;
+        const uint32_t pair = reinterpret_cast<const uint16_t *>(p.cache.scales)[pair_off + h * p.cache.scale_sh];
+        const float sk = scale_value(pair & 0xffu), sv = scale_value(pair >> 8);
+        const int64_t to = b * p.out_sb + t * p.out_st + h * p.out_sh;
+        for (int i = lane; i < p.cache.head_dim; i += 32) {
+            static_cast<T *>(p.k_out)[to + i] = Elem<T>::from_float(decode1<CODE>(p.cache.key[code_off + i]) * sk);
+            static_cast<T *>(p.v_out)[to + i] = Elem<T>::from_float(decode1<CODE>(p.cache.value[code_off + i]) * sv);
+        }
+    }
+}
+
+int lane_shift_of(int dim)
+{
+    int shift = 0;
+    while ((16 << shift) < dim) ++shift;
+    return shift;
 }
 
 struct Launch {
@@ -422,33 +496,37 @@ struct Launch {
     }
 };
 
-unsigned blocks_for(int64_t units, int groups)
+unsigned blocks_for(int64_t units, int per_block)
 {
-    const int64_t per_block = static_cast<int64_t>(groups) * kUnits;
     return static_cast<unsigned>((units + per_block - 1) / per_block);
 }
 
 template <typename T, int CODE> cudaError_t quantize_typed(QuantizeParams p, bool vector, cudaStream_t stream)
 {
-    const int lanes = vector ? lanes_per_row(p.cache.head_dim) : 32;
-    const int groups = kThreads / lanes;
-    p.kv_blocks = static_cast<int>(blocks_for(static_cast<int64_t>(p.tokens) * p.cache.kv_heads, groups));
-    const unsigned q_blocks = p.q_in != nullptr ? blocks_for(static_cast<int64_t>(p.tokens) * p.q_heads, groups) : 0;
+    const int shift = vector ? lane_shift_of(p.cache.head_dim) : 5;
+    const int per_block = (kThreads >> shift) * (vector ? 1 : kScalarUnits);
+    p.kv_div = FastDiv(p.heads_fastest ? p.cache.kv_heads : p.tokens);
+    p.q_div = FastDiv(p.heads_fastest ? std::max(p.q_heads, 1) : p.tokens);
+    p.kv_blocks = static_cast<int>(blocks_for(static_cast<int64_t>(p.tokens) * p.cache.kv_heads, per_block));
+    const unsigned q_blocks = p.q_in != nullptr ? blocks_for(static_cast<int64_t>(p.tokens) * p.q_heads, per_block) : 0;
     Launch rows(dim3(p.kv_blocks + q_blocks, p.batch), kThreads, stream);
-    cudaError_t err = vector ? cudaLaunchKernelEx(&rows.cfg, quantize_vector_kernel<T, CODE>, p, lanes)
-                             : cudaLaunchKernelEx(&rows.cfg, quantize_scalar_kernel<T, CODE>, p);
+    cudaError_t err;
+    if (!vector) err = cudaLaunchKernelEx(&rows.cfg, quantize_scalar_kernel<T, CODE>, p);
+    else if (p.cos != nullptr) err = cudaLaunchKernelEx(&rows.cfg, quantize_vector_kernel<T, CODE, true>, p, shift);
+    else err = cudaLaunchKernelEx(&rows.cfg, quantize_vector_kernel<T, CODE, false>, p, shift);
     if (err != cudaSuccess || p.lens_out == nullptr || p.kv_blocks == 1) return err;
     Launch lengths(dim3(p.batch), 128, stream);
     return cudaLaunchKernelEx(&lengths.cfg, quantize_lengths_kernel, p);
 }
 
-template <typename T, int CODE> cudaError_t dequantize_typed(const DequantizeParams &p, bool vector, cudaStream_t stream)
+template <typename T, int CODE> cudaError_t dequantize_typed(DequantizeParams p, bool vector, cudaStream_t stream)
 {
-    const int lanes = vector ? lanes_per_row(p.cache.head_dim) : 32;
-    const unsigned blocks = blocks_for(static_cast<int64_t>(p.tokens) * p.cache.kv_heads, kThreads / lanes);
-    Launch rows(dim3(blocks, p.batch), kThreads, stream);
-    return vector ? cudaLaunchKernelEx(&rows.cfg, dequantize_kernel<T, CODE, true>, p, lanes)
-                  : cudaLaunchKernelEx(&rows.cfg, dequantize_kernel<T, CODE, false>, p, lanes);
+    const int shift = vector ? lane_shift_of(p.cache.head_dim) : 5;
+    p.div = FastDiv(p.heads_fastest ? p.cache.kv_heads : p.tokens);
+    Launch rows(dim3(blocks_for(static_cast<int64_t>(p.tokens) * p.cache.kv_heads, (kThreads >> shift) * (vector ? 1 : kScalarUnits)), p.batch),
+                kThreads, stream);
+    return vector ? cudaLaunchKernelEx(&rows.cfg, dequantize_vector_kernel<T, CODE>, p, shift)
+                  : cudaLaunchKernelEx(&rows.cfg, dequantize_scalar_kernel<T, CODE>, p);
 }
 
 }  // namespace
