@@ -9,7 +9,9 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 import threading
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 from typing import List, Optional
 
@@ -23,7 +25,6 @@ NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "-shared",
 )
 _LOCK = threading.Lock()
 
@@ -48,6 +49,13 @@ def is_stale() -> bool:
     return any(p.is_file() and p.stat().st_mtime > built for p in deps)
 
 
+def _run(cmd: List[str]) -> str:
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+    return proc.stdout + proc.stderr
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every CUDA source into one shared library; returns its path."""
 
@@ -63,15 +71,15 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         LIB_DIR.mkdir(parents=True, exist_ok=True)
         # One temporary per process: several ranks may find the library stale at the same time.
         tmp = LIB_PATH.with_suffix(f".so.tmp{os.getpid()}")
-        cmd = [nvcc, *NVCC_FLAGS, "-o", str(tmp), *[str(p) for p in source_files()]]
+        with tempfile.TemporaryDirectory() as objects:
+            # The files are independent and the kernels' instances take most of the time: one compiler per core.
+            jobs = [(src, Path(objects) / (src.stem + ".o")) for src in source_files()]
+            verbosity = ["-Xptxas", "-v"] if verbose else []
+            with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+                logs = list(pool.map(lambda job: _run([nvcc, *verbosity, *NVCC_FLAGS, "-c", "-o", str(job[1]), str(job[0])]), jobs))
+            logs.append(_run([nvcc, *NVCC_FLAGS, "-shared", "-o", str(tmp), *[str(obj) for _, obj in jobs]]))
         if verbose:
-            cmd.insert(1, "-Xptxas")
-            cmd.insert(2, "-v")
-        proc = subprocess.run(cmd, capture_output=True, text=True)
-        if proc.returncode != 0:
-            raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
-        if verbose:
-            print(proc.stdout + proc.stderr)
+            print("".join(logs))
         os.replace(tmp, LIB_PATH)
         return LIB_PATH
 

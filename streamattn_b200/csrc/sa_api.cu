@@ -123,8 +123,15 @@ bool encode_map(CUtensorMap *map, int dtype, bool quant, const void *base, const
     cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUtensorMapDataType dt = quant ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : dtype == SA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    // What the L2 fetches around a miss.  8-bit rows of token-major caches are 64 or 128 bytes between other heads' rows,
+    // which the CTA at hand does not want (61 rows of 8192 tokens, Hkv8 D128, pages of 64: 1.53 GB read for 1.03 GB
+    // of cache with 256 bytes).
+    const bool alone = quant && strides[tok_dim - 1] != dims[0];
+    const CUtensorMapL2promotion promotion = !alone          ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                             : dims[0] == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
+                                                             : CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
     CUresult rc = fn(map, dt, 4, const_cast<void *>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     quant && dims[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     quant && dims[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, promotion,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return rc == CUDA_SUCCESS;
 }
@@ -214,6 +221,7 @@ bool build_stream_geometry(const Problem &p, int64_t max_vlen, StreamGeometry *g
         }
     }
     geo->frag_tokens = std::min(unit, tile);
+    if (quant && geo->frag_tokens < tile && strides[2] >= (1ull << 31)) { *why = "pages of 2 GB"; return false; }
     geo->frags_per_tile = tile / geo->frag_tokens;
     geo->frags_per_unit = s.mode == kContig ? 1 : std::max(1, unit / geo->frag_tokens);
     const bool uniform = s.mode == kBlocks || (s.mode == kContig && s.seq_lens == nullptr);

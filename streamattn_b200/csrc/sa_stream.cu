@@ -70,6 +70,8 @@ cudaError_t launch_stream(const Problem &p, const StreamGeometry &geo, const CpF
     sp.first_merges = geo.first_merges;
     sp.seq = p.seq;
     sp.quant = p.quant;
+    sp.key = p.k;
+    sp.value = p.v;
     sp.cp = cp;
 #ifdef SA_TIMELINE
     sp.timeline = g_timeline;

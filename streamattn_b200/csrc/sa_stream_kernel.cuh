@@ -59,6 +59,7 @@ struct StreamParams {
     int first_merges;    // the pair's first CTA merges its split states (no ticket): grids of at most one CTA per SM
     SeqDesc seq;
     QuantScales quant;   // 8-bit caches: where the scale bytes are
+    const void *key, *value;  // ... and the codes, for copies that take no tensor map
     CpFuse cp;           // context-parallel exchange fused into this launch (cp.world == 0: off)
 #ifdef SA_TIMELINE
     unsigned long long *timeline;  // instrumented builds only: 16 words (globaltimer stamps, SM id) per CTA
@@ -165,6 +166,19 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
         ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy)
         : "memory");
+}
+
+// 16 bytes from global to shared memory, asynchronously.
+template <int OFFSET> __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint64_t policy)
+{
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0 + %3], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy), "n"(OFFSET)
+                 : "memory");
+}
+
+// The lane's arrival on `bar` once all of its copy16()s so far have landed.
+__device__ __forceinline__ void arrive_after_copies(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // True on one lane of the (converged) warp.
@@ -579,6 +593,11 @@ __device__ __noinline__ void merge_pair_states(float *first_slot, int64_t slot_s
     __syncthreads();
 }
 
+// Where an instance finds its tokens.  The forms over 8-bit caches are instances of their own - rows in one piece,
+// pages of at least a tile, smaller pages - because their tiles hold half the bytes and what is done once a tile
+// counts twice; 16-bit caches decide at run time.
+enum Place : int { kPlaceAny, kPlaceRows, kPlacePages, kPlaceSmallPages };
+
 // One fragment (TMA box) of a tile as seen by the issuing lane.
 struct Frag {
     int x;              // global tile index, -1: no tile (warp-uniform)
@@ -587,14 +606,16 @@ struct Frag {
     int outer;          // outermost coordinate: batch row or physical page
     int kvh;            // kv head coordinate
     int64_t trace_idx;  // slot of the page-walk trace to record, or -1
+    uint32_t page[2];   // 8-bit caches: the page table's entry as it was loaded, not yet looked at
 };
 
-template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE>
+template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ StreamParams p)
 {
     constexpr bool QUANT = CODE != kCodeNone;
+    constexpr bool PAGED = PLACE == kPlacePages || PLACE == kPlaceSmallPages;  // 8-bit caches only
     constexpr int TILE_N = QUANT ? quant_tile_tokens(D) : kTileBytes / (D * 2);  // tokens per tile
     constexpr int TILE_BYTES = QUANT ? TILE_N * D : kTileBytes;              // one K or one V tile
     constexpr int STAGE_BYTES = 2 * TILE_BYTES;
@@ -651,7 +672,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     }
     if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < STAGES; ++s) mbar_init(bar_u32 + s * 8, 1);
+        for (int s = 0; s < STAGES; ++s) mbar_init(bar_u32 + s * 8, PLACE == kPlaceSmallPages ? 32 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Programmatic dependent launch: let the next kernel of the stream be scheduled as this
@@ -972,7 +993,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     }
     auto lookup = [&](int x) -> Frag {
         Frag f;
-        f.x = x; f.state = 0; f.tok = 0; f.outer = 0; f.kvh = 0; f.trace_idx = -1;
+        f.x = x; f.state = 0; f.tok = 0; f.outer = 0; f.kvh = 0; f.trace_idx = -1; f.page[0] = f.page[1] = 0;
         if (x < 0) return f;
         if (x >= pc_end) {
             int b, row_tiles;
@@ -985,18 +1006,23 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if constexpr (QUANT) {
             f.kvh = pc_head;
             const int tok = (x - pc_start) * TILE_N + (lane << p.frag_shift);
-            const bool mine = lane < p.frags_per_tile && tok < static_cast<int>(pc_vlen);
+            const bool mine = lane < (PLACE == kPlaceSmallPages ? p.frags_per_tile : 1) && tok < static_cast<int>(pc_vlen);
             f.tok = tok;
             f.outer = pc_b;
             f.state = mine;
-            if (p.seq.mode == kPaged && mine) {
+            if (PAGED && mine) {
                 const int page_shift = p.fpu_shift + p.frag_shift;
                 const int lp = tok >> page_shift;
                 const int64_t slot = static_cast<int64_t>(pc_b) * p.seq.max_pages + lp;
-                const int64_t page = load_index(p.seq.page_table, p.seq.table_i64, slot);
+                // Nothing may depend on the entry here, or the warp waits for it before it turns to its next tile.
+                if (p.seq.table_i64) {
+                    const uint2 entry = static_cast<const uint2 *>(p.seq.page_table)[slot];
+                    f.page[0] = entry.x;
+                    f.page[1] = entry.y;
+                } else {
+                    f.page[0] = static_cast<const uint32_t *>(p.seq.page_table)[slot];
+                }
                 f.tok = tok - (lp << page_shift);
-                f.outer = static_cast<int>(page);
-                f.state = (page >= 0 && page < p.seq.num_pages) ? 1 : 2;
                 if (pc_kvh == 0 && f.tok == 0) f.trace_idx = slot;
             }
             return f;
@@ -1039,38 +1065,65 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 
     // Issue the TMA copies of the warp's j-th tile into ring slot j % STAGES.  Returns the set of
     // its fragments that are left out because their page id is out of range.
-    auto issue = [&](int j, const Frag &f) -> unsigned {
+    auto issue = [&](int j, Frag f) -> unsigned {
         const uint32_t slot = static_cast<uint32_t>(j) % STAGES;
         const uint32_t stage = ring_u32 + slot * STAGE_BYTES;
         const uint32_t bar = bar_u32 + slot * 8;
+        if (PAGED && f.state == 1) {
+            const int64_t page = p.seq.table_i64
+                                     ? static_cast<int64_t>(static_cast<uint64_t>(f.page[1]) << 32 | f.page[0])
+                                     : static_cast<int64_t>(static_cast<int32_t>(f.page[0]));
+            f.outer = static_cast<int>(page);
+            f.state = (page >= 0 && page < p.seq.num_pages) ? 1 : 2;
+        }
         const bool ok = f.state == 1;
         if (f.state == 2) atomicOr(p.status, SA_DEV_BAD_PAGE);
-        if (ok && p.trace != nullptr && f.trace_idx >= 0) p.trace[f.trace_idx] = static_cast<int32_t>(f.outer);
+        if ((!QUANT || PAGED) && ok && p.trace != nullptr && f.trace_idx >= 0) p.trace[f.trace_idx] = static_cast<int32_t>(f.outer);
         const unsigned mask = __ballot_sync(0xffffffffu, ok);
         if constexpr (QUANT) {
-            // One elected lane issues the fragments one after the other: copies take their operands from uniform
-            // registers, and a lane each (below) is served by a loop over the lanes for every one of the
-            // three copies (measured with pages of 16, four fragments a tile: 39.3 instead of 40.6 us for 136 MB).
             const unsigned bad = __ballot_sync(0xffffffffu, f.state == 2);
-            const bool leader = elect_one();
             const int frag = p.frag_tokens;
-            int scale_bytes = 2 * frag;  // of a fragment: a page has them all, a row ends at the cache's capacity
-            if (p.seq.mode == kContig) {
-                const int room = static_cast<int>(p.seq.kv_len) - (f.tok - lane * frag);  // lane 0's fragment
-                scale_bytes = 2 * (room < frag ? room : frag);
+            if constexpr (PLACE == kPlaceSmallPages) {
+                // Pages smaller than a tile: 16 bytes a lane and copy, the swizzle applied here.  What is not to be
+                // loaded (a bad page, tokens behind the row) takes page 0's place: it is masked when it is used.
+                constexpr int CHUNKS = D / 16, ROWS_PER = 32 / CHUNKS;  // pieces of a row, rows of one warp-wide copy
+                const int r0 = lane / CHUNKS, chunk = lane % CHUNKS;
+                const int page_stride = static_cast<int>(p.seq.pg_sp), row_stride = static_cast<int>(p.seq.pg_st);
+                const uint8_t *k_lane = static_cast<const uint8_t *>(p.key) + f.kvh * p.seq.pg_sh + r0 * row_stride + chunk * 16;
+                const int64_t to_value = static_cast<const uint8_t *>(p.value) - static_cast<const uint8_t *>(p.key);
+                const int page_of = f.state == 1 ? f.outer : 0;
+                const uint32_t dst = stage + piece<D>(r0, chunk);
+                unrolled<TILE_N / ROWS_PER>([&](auto it_c) {
+                    constexpr int row = decltype(it_c)::value * ROWS_PER;
+                    const int page = __shfl_sync(0xffffffffu, page_of, row >> p.frag_shift);
+                    const uint8_t *src = k_lane + static_cast<int64_t>(page) * page_stride +
+                                         static_cast<int64_t>(row & (frag - 1)) * row_stride;
+                    // D = 128: rows r + 4 .. r + 7 have the other half of the swizzle.
+                    const uint32_t to = (D == 128 && (row & 4)) ? dst ^ 64 : dst;
+                    copy16<row * D>(to, src, policy);
+                    copy16<row * D + TILE_BYTES>(to, src + to_value, policy);
+                });
+                // Scale pairs: 8 tokens a lane.
+                const int page = __shfl_sync(0xffffffffu, page_of, (lane * 8) >> p.frag_shift);
+                if (lane < TILE_N / 8)
+                    copy16<0>(scale_u32 + slot * SCALE_BYTES + lane * 16,
+                              p.quant.scales + 2 * (page * p.quant.so + f.kvh * p.quant.sh + ((lane * 8) & (frag - 1))), policy);
+                arrive_after_copies(bar);
+                return bad;
             }
-            if (leader) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(__popc(mask) * (frag * D * 2 + scale_bytes)));
-            for (unsigned left = mask; left != 0u; left &= left - 1) {
-                const int i = __ffs(left) - 1;
-                const int tok = __shfl_sync(0xffffffffu, f.tok, i);
-                const int outer = __shfl_sync(0xffffffffu, f.outer, i);
-                if (leader) {
-                    const uint32_t dst = stage + i * frag * D;
+            // One box a tile: the whole of it, or a part of a page (whose sizes are powers of two).
+            const int tok = __shfl_sync(0xffffffffu, f.tok, 0);
+            const int outer = __shfl_sync(0xffffffffu, f.outer, 0);
+            if (elect_one()) {
+                int scale_bytes = TILE_N * 2;  // a page has them all, a contiguous row ends at the cache's capacity
+                if (!PAGED && static_cast<int>(p.seq.kv_len) - tok < TILE_N) scale_bytes = 2 * (static_cast<int>(p.seq.kv_len) - tok);
+                mbar_arrive_expect_tx(bar, mask != 0u ? static_cast<uint32_t>(2 * TILE_BYTES + scale_bytes) : 0u);
+                if (mask != 0u) {
                     const int c1 = p.tok_dim == 1 ? tok : f.kvh;
                     const int c2 = p.tok_dim == 1 ? f.kvh : tok;
-                    tma_load_4d(dst, &tm_k, bar, 0, c1, c2, outer, policy);
-                    tma_load_4d(dst + TILE_BYTES, &tm_v, bar, 0, c1, c2, outer, policy);
-                    bulk_load(scale_u32 + slot * SCALE_BYTES + i * frag * 2,
+                    tma_load_4d(stage, &tm_k, bar, 0, c1, c2, outer, policy);
+                    tma_load_4d(stage + TILE_BYTES, &tm_v, bar, 0, c1, c2, outer, policy);
+                    bulk_load(scale_u32 + slot * SCALE_BYTES,
                               p.quant.scales + 2 * (outer * p.quant.so + f.kvh * p.quant.sh + tok), scale_bytes, bar, policy);
                 }
             }
@@ -1574,11 +1627,11 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     }
 }
 
-template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE>
+template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE>
 cudaError_t launch_instance(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int ctas,
                             int batch, cudaStream_t stream)
 {
-    auto kernel = stream_decode_kernel<T, D, WARPS, STAGES, ROWS16, CODE>;
+    auto kernel = stream_decode_kernel<T, D, WARPS, STAGES, ROWS16, CODE, PLACE>;
     const size_t smem = stream_smem_bytes(D, ROWS16, STAGES, batch, CODE != kCodeNone);
     // Opt in to the dynamic shared memory this launch needs (grows only; per device).
     static std::mutex mu;
@@ -1610,26 +1663,33 @@ cudaError_t launch_instance(const CUtensorMap &mk, const CUtensorMap &mv, const 
     return cudaLaunchKernelEx(&cfg, kernel, mk, mv, sp);
 }
 
-template <typename T, int D, int CODE>
-cudaError_t launch_dim(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int ctas, int batch,
-                       bool rows16, cudaStream_t stream)
+template <typename T, int D, int CODE, int PLACE>
+cudaError_t launch_place(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int ctas, cudaStream_t stream)
 {
     constexpr bool kQuant = CODE != kCodeNone;
-    if (rows16)
-        return launch_instance<T, D, warps_of(D, true, kQuant), stages_of(D, true, kQuant), true, CODE>(mk, mv, sp, ctas, batch, stream);
-    return launch_instance<T, D, warps_of(D, false, kQuant), stages_of(D, false, kQuant), false, CODE>(mk, mv, sp, ctas, batch, stream);
+    if (sp.group > 8)
+        return launch_instance<T, D, warps_of(D, true, kQuant), stages_of(D, true, kQuant), true, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
+    return launch_instance<T, D, warps_of(D, false, kQuant), stages_of(D, false, kQuant), false, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
+}
+
+template <typename T, int D, int CODE>
+cudaError_t launch_dim(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int ctas, cudaStream_t stream)
+{
+    if constexpr (CODE == kCodeNone) return launch_place<T, D, CODE, kPlaceAny>(mk, mv, sp, ctas, stream);
+    else if (sp.seq.mode == kContig) return launch_place<T, D, CODE, kPlaceRows>(mk, mv, sp, ctas, stream);
+    else if (sp.frags_per_tile == 1) return launch_place<T, D, CODE, kPlacePages>(mk, mv, sp, ctas, stream);
+    else return launch_place<T, D, CODE, kPlaceSmallPages>(mk, mv, sp, ctas, stream);
 }
 
 template <int CODE>
 cudaError_t launch_code(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int dtype, int head_dim,
                         int ctas, cudaStream_t stream)
 {
-    const bool rows16 = sp.group > 8;
     if (dtype == SA_DTYPE_BF16)
-        return head_dim == 64 ? launch_dim<__nv_bfloat16, 64, CODE>(mk, mv, sp, ctas, sp.batch, rows16, stream)
-                              : launch_dim<__nv_bfloat16, 128, CODE>(mk, mv, sp, ctas, sp.batch, rows16, stream);
-    return head_dim == 64 ? launch_dim<__half, 64, CODE>(mk, mv, sp, ctas, sp.batch, rows16, stream)
-                          : launch_dim<__half, 128, CODE>(mk, mv, sp, ctas, sp.batch, rows16, stream);
+        return head_dim == 64 ? launch_dim<__nv_bfloat16, 64, CODE>(mk, mv, sp, ctas, stream)
+                              : launch_dim<__nv_bfloat16, 128, CODE>(mk, mv, sp, ctas, stream);
+    return head_dim == 64 ? launch_dim<__half, 64, CODE>(mk, mv, sp, ctas, stream)
+                          : launch_dim<__half, 128, CODE>(mk, mv, sp, ctas, stream);
 }
 
 }  // namespace
