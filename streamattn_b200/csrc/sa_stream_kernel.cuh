@@ -606,7 +606,6 @@ struct Frag {
     int outer;          // outermost coordinate: batch row or physical page
     int kvh;            // kv head coordinate
     int64_t trace_idx;  // slot of the page-walk trace to record, or -1
-    uint32_t page[2];   // 8-bit caches: the page table's entry as it was loaded, not yet looked at
 };
 
 template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE>
@@ -983,6 +982,10 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     int pc_b = -1, pc_kvh = 0, pc_start = 0, pc_end = 0;
     int64_t pc_vlen = 0;
     int pc_head = 0;  // 8-bit caches: the cache's own head index of pc_kvh
+    // ... and, paged: the page table's entries of the warp's next tiles, 32 at a time, a tile's fragments side by side.  One
+    // load a tile would hold the warp up for its latency every time (N = 262144 in pages of 64: 98.8 us, 87.8 without it).
+    uint32_t entry[2] = {0u, 0u};
+    int entry_at = 32;  // lane that holds the next tile's first entry; 32: none left
     if (aligned && hi > lo) {  // all of this CTA's tiles belong to one pair: no search needed
         pc_b = al_pair / Hkv;
         pc_kvh = al_pair - pc_b * Hkv;
@@ -993,7 +996,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     }
     auto lookup = [&](int x) -> Frag {
         Frag f;
-        f.x = x; f.state = 0; f.tok = 0; f.outer = 0; f.kvh = 0; f.trace_idx = -1; f.page[0] = f.page[1] = 0;
+        f.x = x; f.state = 0; f.tok = 0; f.outer = 0; f.kvh = 0; f.trace_idx = -1;
         if (x < 0) return f;
         if (x >= pc_end) {
             int b, row_tiles;
@@ -1002,6 +1005,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             if (b != pc_b) pc_vlen = vlen_of(b);
             pc_b = b;
             pc_head = pc_kvh / p.kv_split;
+            entry_at = 32;
         }
         if constexpr (QUANT) {
             f.kvh = pc_head;
@@ -1010,20 +1014,37 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             f.tok = tok;
             f.outer = pc_b;
             f.state = mine;
-            if (PAGED && mine) {
+            if constexpr (PAGED) {
                 const int page_shift = p.fpu_shift + p.frag_shift;
-                const int lp = tok >> page_shift;
-                const int64_t slot = static_cast<int64_t>(pc_b) * p.seq.max_pages + lp;
-                // Nothing may depend on the entry here, or the warp waits for it before it turns to its next tile.
-                if (p.seq.table_i64) {
-                    const uint2 entry = static_cast<const uint2 *>(p.seq.page_table)[slot];
-                    f.page[0] = entry.x;
-                    f.page[1] = entry.y;
-                } else {
-                    f.page[0] = static_cast<const uint32_t *>(p.seq.page_table)[slot];
+                const int fpt_shift = PLACE == kPlaceSmallPages ? p.fpt_shift : 0;
+                const int64_t row = static_cast<int64_t>(pc_b) * p.seq.max_pages;
+                if (entry_at == 32) {
+                    const int xa = x + (lane >> fpt_shift) * step;
+                    const int at = (xa - pc_start) * TILE_N + ((lane & ((1 << fpt_shift) - 1)) << p.frag_shift);
+                    if (xa < pc_end && at < static_cast<int>(pc_vlen)) {
+                        const int64_t slot = row + (at >> page_shift);
+                        if (p.seq.table_i64) {
+                            const uint2 e = static_cast<const uint2 *>(p.seq.page_table)[slot];
+                            entry[0] = e.x;
+                            entry[1] = e.y;
+                        } else {
+                            entry[0] = static_cast<const uint32_t *>(p.seq.page_table)[slot];
+                            entry[1] = static_cast<int32_t>(entry[0]) < 0 ? 0xffffffffu : 0u;
+                        }
+                    }
+                    entry_at = 0;
                 }
-                f.tok = tok - (lp << page_shift);
-                if (pc_kvh == 0 && f.tok == 0) f.trace_idx = slot;
+                const uint32_t low = __shfl_sync(0xffffffffu, entry[0], entry_at + lane);
+                const uint32_t high = __shfl_sync(0xffffffffu, entry[1], entry_at + lane);
+                entry_at += 1 << fpt_shift;
+                if (mine) {
+                    const int64_t page = static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+                    const int lp = tok >> page_shift;
+                    f.tok = tok - (lp << page_shift);
+                    f.outer = static_cast<int>(low);
+                    f.state = (page >= 0 && page < p.seq.num_pages) ? 1 : 2;
+                    if (pc_kvh == 0 && f.tok == 0) f.trace_idx = row + lp;
+                }
             }
             return f;
         }
@@ -1065,17 +1086,10 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 
     // Issue the TMA copies of the warp's j-th tile into ring slot j % STAGES.  Returns the set of
     // its fragments that are left out because their page id is out of range.
-    auto issue = [&](int j, Frag f) -> unsigned {
+    auto issue = [&](int j, const Frag &f) -> unsigned {
         const uint32_t slot = static_cast<uint32_t>(j) % STAGES;
         const uint32_t stage = ring_u32 + slot * STAGE_BYTES;
         const uint32_t bar = bar_u32 + slot * 8;
-        if (PAGED && f.state == 1) {
-            const int64_t page = p.seq.table_i64
-                                     ? static_cast<int64_t>(static_cast<uint64_t>(f.page[1]) << 32 | f.page[0])
-                                     : static_cast<int64_t>(static_cast<int32_t>(f.page[0]));
-            f.outer = static_cast<int>(page);
-            f.state = (page >= 0 && page < p.seq.num_pages) ? 1 : 2;
-        }
         const bool ok = f.state == 1;
         if (f.state == 2) atomicOr(p.status, SA_DEV_BAD_PAGE);
         if ((!QUANT || PAGED) && ok && p.trace != nullptr && f.trace_idx >= 0) p.trace[f.trace_idx] = static_cast<int32_t>(f.outer);
