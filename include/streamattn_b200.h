@@ -474,8 +474,8 @@ typedef struct sa_quant_cache {
  *   lens_out       optional device array [batch] (type of positions): position + count; may be the
  *                  per-row `positions` itself
  *   cos, sin       optional [batch or 1, tokens, D], dtype `dtype` (rope_stride_b = 0: shared)
- *   q_in / q_out   optional [batch, tokens, q_heads, D]: the query rotated (fp32, rounded once) or,
- *                  without cos / sin, copied; q_out must not alias q_in
+ *   q_in / q_out   optional [batch, tokens, q_heads, D]: the query of all tokens, padding included,
+ *                  rotated (fp32, rounded once) or, without cos / sin, copied; q_out must not alias q_in
  *   status         optional device int32.  A row whose tokens do not fit the cache is left out as a
  *                  whole (SA_DEV_BAD_POSITION), a token whose page id is out of range is skipped
  *                  (SA_DEV_BAD_PAGE); in both cases the row's entry of lens_out is not written.

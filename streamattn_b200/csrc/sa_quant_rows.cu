@@ -221,8 +221,7 @@ __global__ void __launch_bounds__(kThreads) quantize_vector_kernel(const __grid_
     float x[8], y[8];
 
     if (is_query) {
-        const int count = clipped_count(p.counts, p.counts_i64, b, p.tokens);
-        if (unit >= static_cast<unsigned>(p.tokens) * p.q_heads || t >= count || !in_row) return;
+        if (unit >= static_cast<unsigned>(p.tokens) * p.q_heads || !in_row) return;
         Halves<T> q;
         q.load(static_cast<const T *>(p.q_in) + b * p.qi_sb + at(t, p.qi_st) + at(h, p.qi_sh) + d, half);
         if (ROPE) {
@@ -302,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) quantize_scalar_kernel(const __grid_
     const bool rope = p.cos != nullptr;
     const bool is_query = static_cast<int>(blockIdx.x) >= p.kv_blocks;
     // The query's CTAs must not read the position: another CTA may be replacing it.
-    const RowPlace place = is_query ? RowPlace{0, clipped_count(p.counts, p.counts_i64, b, p.tokens), true} : row_place(p, b);
+    const RowPlace place = is_query ? RowPlace{0, p.tokens, true} : row_place(p, b);
     const int heads = is_query ? p.q_heads : p.cache.kv_heads;
     const unsigned total = static_cast<unsigned>(p.tokens) * heads;
     const unsigned first = (blockIdx.x - (is_query ? p.kv_blocks : 0)) * kWarps * kScalarUnits + warp;

@@ -166,7 +166,8 @@ def quantize_kv(cache: QuantCache, key_new: torch.Tensor, value_new: torch.Tenso
     With ``cos``/``sin`` (``[B or 1, T, D]`` in the rows' dtype; ``[B or 1, D]`` for one token) K is rotated,
     ``x * cos + rotate_half(x) * sin`` in fp32, and quantised without being rounded in between.  ``query``
     (``[B, T, Hq, D]``, or ``query_layout="BHND"``) is rotated likewise, rounded once, into ``query_out``,
-    which is returned; without ``cos``/``sin`` it is copied.
+    which is returned; without ``cos``/``sin`` it is copied.  All ``T`` tokens of it are, whatever ``counts``
+    says, so that no row of ``query_out`` is left undefined.
 
     ``status`` (device int32) collects ``SA_DEV_BAD_POSITION`` for rows whose tokens do not fit the
     cache - such a row is left out as a whole - and ``SA_DEV_BAD_PAGE`` for tokens whose page is not

@@ -118,11 +118,7 @@ def test_write_gives_the_oracles_bytes_and_nothing_else(dev, case, ragged):
     assert int(status) == 0 and lengths.tolist() == [s + n for s, n in zip(starts, counts)]
     assert positions.tolist() == starts and cache.sequence_lengths.tolist() == [0] * B
     if rope:
-        want = torch.full_like(q, 7.0)                       # the query's padding is left alone as well
-        turned = oracle.rotate(q, cos, sin).to(dtype)
-        for b in range(B):
-            want[b, :counts[b]] = turned[b, :counts[b]]
-        assert got is out and torch.equal(got.cpu(), want)
+        assert got is out and torch.equal(got.cpu(), oracle.rotate(q, cos, sin).to(dtype))   # padding as well
 
 
 @pytest.mark.parametrize("code", list(CODES))
