@@ -115,6 +115,8 @@ class QuantizeKVPlan(AppendKVPlan):
             raise ValueError("positions must have the dtype of the lengths that are written")
         pos_dtype, num_positions = _positions(positions, batch, lengths_out)
         counts_dtype = _optional_counts(counts, batch, "counts")
+        if any(st == 0 and n > 1 for t in (cache.key, cache.value, cache.scales) for st, n in zip(t.stride(), t.shape)):
+            raise ValueError("the rows of a cache that is written must not share memory")
         if lengths_out is not None and counts is not None and lengths_out.data_ptr() == counts.data_ptr():
             raise ValueError("counts must not alias the lengths that are written")
         cos, sin, rope_strides = _angles(cos, sin, batch, tokens, dim, dtype)

@@ -144,6 +144,9 @@ def test_aliased_lengths_and_missing_lengths_are_refused():
         sa.quantize_kv(contig(lens=False), K, K, positions=torch.zeros(2, dtype=torch.int32), advance_lengths=True)
     with pytest.raises(ValueError, match="QuantKVCache"):
         sa.quantize_kv(K, K, K)
+    shared = torch.zeros(1, 4, 16, 64, dtype=torch.int8).expand(2, 4, 16, 64)
+    with pytest.raises(ValueError, match="must not share memory"):
+        sa.quantize_kv(contig(key=shared, value=shared), K, K)
 
 
 @pytest.mark.parametrize("kwargs,match", [
