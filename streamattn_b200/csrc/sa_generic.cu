@@ -86,9 +86,16 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
     const KV *kbase = static_cast<const KV *>(p.k);
     const KV *vbase = static_cast<const KV *>(p.v);
 
-    for (int d = threadIdx.x; d < dim; d += kGenericThreads)
-        sm_q[d] = Elem<T>::to_float(q[d]) * p.scale_log2;
-    __syncthreads();
+    bool nan_row = false;  // 8-bit caches: a token whose scale is NaN, or such a query, makes the result NaN
+    for (int d = threadIdx.x; d < dim; d += kGenericThreads) {
+        float x = Elem<T>::to_float(q[d]);
+        if (CODE != kCodeNone && (__float_as_uint(x) & 0x7fffffffu) >= 0x7f800000u) {
+            nan_row = true;
+            x = 0.0f;
+        }
+        sm_q[d] = x * p.scale_log2;
+    }
+    if (CODE != kCodeNone) nan_row = __syncthreads_or(nan_row); else __syncthreads();
 
     const int64_t vlen = row_vlen(p.seq, b);
     int64_t chunk = (vlen + p.splits - 1) / p.splits;
@@ -100,7 +107,6 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
     float o[kMaxDim / 32];
 #pragma unroll
     for (int i = 0; i < kMaxDim / 32; ++i) o[i] = 0.0f;
-    bool nan_row = false;  // 8-bit caches: a token whose scale is NaN makes the result NaN
 
     for (int64_t blk = t_begin + warp * 32; blk < t_end; blk += kGenericWarps * 32) {
         const int64_t t = blk + lane;

@@ -753,7 +753,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         // 8-bit caches: a second segment costs a CTA about as much as a round of its warps' tiles (3 us).  With
         // n = floor(C / pairs) CTAs for the pairs that get fewest, an aligned CTA takes C / (n pairs) times the T / (C WARPS)
         // rounds of an equal slice; while that is at most 1.2 rounds more, the CTAs are aligned, and if a ragged pair's
-        // share comes out at none, every pair gets one (128 pairs of 512 tokens, D128: 10.6 -> 7.1 us, of 2048: @@;
+        // share comes out at none, every pair gets one (128 pairs of 512 tokens, D128: 10.6 -> 7.1 us, of 2048: 18.7 -> 14.2;
         // 126 ragged ones of 132 to 526: 16.7 -> 9.7 us).
         const int64_t fewest = num_pairs <= C ? static_cast<int64_t>(C / num_pairs) * num_pairs : 0;
         const bool short_rows = QUANT && fewest > 0 &&
@@ -1045,8 +1045,8 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 const int64_t row = static_cast<int64_t>(pc_b) * p.seq.max_pages;
                 if (entry_at == 32) {
                     const int xa = x + (lane >> fpt_shift) * step;
-                    const int at = (xa - pc_start) * TILE_N + ((lane & ((1 << fpt_shift) - 1)) << p.frag_shift);
-                    if (xa < pc_end && at < static_cast<int>(pc_vlen)) {
+                    const int at = xa < pc_end ? (xa - pc_start) * TILE_N + ((lane & ((1 << fpt_shift) - 1)) << p.frag_shift) : -1;
+                    if (at >= 0 && at < static_cast<int>(pc_vlen)) {
                         const int64_t slot = row + (at >> page_shift);
                         if (p.seq.table_i64) {
                             const uint2 e = static_cast<const uint2 *>(p.seq.page_table)[slot];

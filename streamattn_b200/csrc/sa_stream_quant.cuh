@@ -170,12 +170,14 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
     float o[NH][DT][4];          // in units of 2^(v_exp - 142)
     int v_exp;                   // largest scale byte of V so far, at least 16
     bool has_nan;                // a NaN scale was met: the result is NaN
+    int nan_heads;               // bit 2 nh + h: the query of that head holds a NaN or an infinity, and its result is NaN
 
     // Query rows of `group` heads from head0 on; lane (g, t4) holds columns of head g of each eight.
     __device__ __forceinline__ void begin(const T *q0, int64_t stride, int group, float scale_log2, int g, int t4)
     {
         v_exp = 16;
         has_nan = false;
+        nan_heads = 0;
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
             const bool ok = nh * 8 + g < group;
@@ -196,13 +198,21 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
             }
             amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // m and l stay finite, as for NaN scales, so that no merge takes the state for an empty one.
+            const bool finite = amax < 0x7f800000u;
+            if (!finite) {
+                amax = 0;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
+            }
             float scale;
             if constexpr (CODE == kCodeE4M3) {
                 // Exponent of the factor: at least -113, and at most 100 to keep the scale clear of zero.
                 const int up = amax == 0 ? 0 : min(14 + 127 - static_cast<int>(amax >> 23), 100);
                 const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-                scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu)   // a NaN or an infinity: NaN
-                                            : scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+                scale = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
                 // A 32-bit word of K codes c0 .. c3 becomes the halves c0 c1 and c2 c3; a lane's word 4 t4 .. of the first
                 // 16 bytes of a k-step meets the lane's word of the second 16 bytes in one instruction each.
 #pragma unroll
@@ -215,7 +225,7 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
             } else {
                 const float big = fmaxf(__uint_as_float(amax), __uint_as_float(27u << 23));
                 const float inv = 32512.0f / big;
-                scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : scale_log2 * (big * (1.0f / 32512.0f));
+                scale = scale_log2 * (big * (1.0f / 32512.0f));
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -233,6 +243,7 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
             }
             row_scale[nh][0] = __shfl_sync(0xffffffffu, scale, 8 * t4);
             row_scale[nh][1] = __shfl_sync(0xffffffffu, scale, 8 * t4 + 4);
+            nan_heads |= (__shfl_sync(0xffffffffu, finite ? 0 : 1, 8 * t4) | __shfl_sync(0xffffffffu, finite ? 0 : 2, 8 * t4 + 4)) << (2 * nh);
             m[nh][0] = m[nh][1] = -INFINITY;
             l[nh][0] = l[nh][1] = 0.0f;
 #pragma unroll
@@ -480,7 +491,7 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
                 for (int i = 0; i < DT; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        row[g * (D / 8) + 2 * i + e] = has_nan ? __uint_as_float(0x7fffffffu) : o[nh][i][2 * e + h] * unit;
+                        row[g * (D / 8) + 2 * i + e] = has_nan || ((nan_heads >> (2 * nh + h)) & 1) ? __uint_as_float(0x7fffffffu) : o[nh][i][2 * e + h] * unit;
                 if (g == 0) {
                     row[D] = m[nh][h] * row_scale[nh][h];
                     row[D + 1] = sum;

@@ -150,6 +150,50 @@ def test_nan_rows_reach_their_head_and_no_other(dev, kernel):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("code", list(CODES))
+def test_nan_and_infinite_queries_make_their_head_nan(dev, kernel, code):
+    B, H, G, D, lengths = 2, 1, 11, 64, [300, 0]
+    cache, mirror = filled(dev, "contig", "BHND", code, B, H, D, 320, lengths, seed=6)
+    q = new_rows((B, 1, H * G, D), torch.bfloat16, 3).clamp(-30, 30)
+    q[0, 0, 2, 5], q[0, 0, 9, 63], q[0, 0, 10, 0], q[1, 0, 0, 0] = float("nan"), float("inf"), -float("inf"), float("nan")
+    bad = [2, 9, 10]
+    for splits in (None, 1, 4):
+        plan = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel, splits=splits)
+        out = plan.run().cpu()
+        assert bool(torch.isnan(out[0, 0, bad]).all()) and not bool(out[1].any())      # a row of no tokens is zero
+        good = [h for h in range(G) if h not in bad]
+        want, spread, reach = oracle.attend(q[:, :, good], mirror, lengths)
+        tol = tolerance(want, spread, reach, q.dtype, D, 300)
+        assert bool(((out[:, :, good].double() - want).abs() <= tol).all())
+    state = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel, return_state=True).run().cpu()
+    assert bool(torch.isfinite(state[0, :, D:]).all()) and bool(torch.isnan(state[0, bad, :D]).all())
+
+
+def test_offsets_beyond_32_bits(dev):
+    """A row whose codes pass 2^32 bytes: written, attended to and read back at its far end."""
+    H, D, N, T = 16, 128, 2 ** 21 + 128, 70
+    cache = sa.QuantKVCache.empty(1, H, N, D, device=dev)                 # 4.3 GB each of K and V
+    cache.scales.fill_(100)
+    k = torch.full((1, T, H, D), 4.0, device=dev).bfloat16()
+    v = torch.randn(1, T, H, D, generator=torch.Generator(dev).manual_seed(1), device=dev).bfloat16()
+    start = torch.full((1,), N - T, dtype=torch.int64, device=dev)
+    lens = torch.zeros(1, dtype=torch.int64, device=dev)
+    sa.quantize_kv(cache, k, v, positions=start, lengths_out=lens)
+    assert int(lens) == N
+    key, value = sa.dequantize_kv(cache, tokens=T, starts=start, dtype=torch.float32)
+    assert torch.equal(key, k.float())
+    bound = torch.maximum(v.float().abs() * 2 ** -4, v.float().abs().amax(-1, keepdim=True) / 224 * 2 ** -10)
+    assert bool(((value - v.float()).abs() <= bound).all())
+    # q . k / sqrt(D) = 4 * D / sqrt(D) = 45 for the T last tokens and 0 for all others: e^-45 of 2^21 tokens is nothing
+    q = torch.ones(1, 1, H * 4, D, device=dev).bfloat16()
+    cache.sequence_lengths.fill_(N)
+    out = sa.stream_attn_quant_decode(q, cache)
+    want = value[0].double().mean(0).repeat_interleave(4, dim=0)
+    spread = value[0].double().abs().mean(0).repeat_interleave(4, dim=0)
+    assert bool(((out[0, 0].double() - want).abs() <= 2 ** -8 * want.abs() + spread * (2 ** -11 + 2 ** -15)).all())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page", [8, 16, 64, 128])
 def test_bad_pages_are_left_out_and_reported(dev, kernel, page, dim):
@@ -252,6 +296,36 @@ def test_pinned_query_and_output(dev):
     plan.run()
     torch.cuda.synchronize()
     check(out, q, mirror, lengths)
+
+
+@pytest.mark.parametrize("batch,heads,capacity,low", [(40, 3, 256, 1), (63, 2, 1024, 100), (20, 8, 512, 0), (9, 8, 640, 400)])
+@pytest.mark.parametrize("page", [0, 16, 64])
+def test_many_short_rows(dev, batch, heads, capacity, low, page):
+    """Around one CTA a (row, KV head) pair: aligned slices, one CTA each, and slices across pairs give the same."""
+    D, G = 64, 4
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(low, capacity + 1, (batch,), generator=g)
+    cache = sa.QuantKVCache.empty(batch, heads, capacity, D, device=dev)
+    k, v = (torch.randn(batch, capacity, heads, D, generator=g).bfloat16().to(dev) for _ in range(2))
+    sa.quantize_kv(cache, k, v, counts=lengths.to(dev))
+    key, value = (x.transpose(1, 2).double() for x in sa.dequantize_kv(cache, dtype=torch.float32))    # [B, H, N, D]
+    if page:
+        paged = sa.QuantPagedKVCache.empty(batch * capacity // page, page, heads, D, batch=batch,
+                                           max_pages_per_request=capacity // page, device=dev)
+        paged.page_table.copy_(torch.randperm(batch * capacity // page, generator=g).view(batch, -1))
+        sa.quantize_kv(paged, k, v, counts=lengths.to(dev))
+        cache = paged
+    q = torch.randn(batch, 1, heads * G, D, generator=g).bfloat16().to(dev)
+    qh = q[:, 0].double().view(batch, heads, G, D)
+    scores = qh @ key.transpose(2, 3) / D ** 0.5
+    mask = torch.arange(capacity, device=dev)[None, None, None] >= lengths.to(dev)[:, None, None, None]
+    p = torch.softmax(scores.masked_fill(mask, -1e300), -1).masked_fill(mask, 0.0)
+    want, spread = p @ value, p @ value.abs()
+    reach = (qh.abs() @ key.abs().transpose(2, 3)).masked_fill(mask, 0.0).amax(-1, keepdim=True) / D ** 0.5
+    tol = tolerance(want, spread, reach, q.dtype, D, capacity)
+    for splits in (None, 1, 3):
+        got = sa.QuantDecodePlan.build(q, cache, splits=splits).run().double().view_as(want)
+        assert bool(((got - want).abs() <= tol).all()), (splits, float(((got - want).abs() - tol).max()))
 
 
 def test_strided_query_and_views_of_larger_caches(dev):
