@@ -55,6 +55,19 @@ def _optional_counts(t: Optional[torch.Tensor], batch: int, name: str) -> int:
     return native.SA_INDEX[t.dtype]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+
+    return a.device == b.device and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() \
+        and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def _folded(t: torch.Tensor) -> bool:
+    """Whether entries along an axis are the same memory (an expanded tensor)."""
+
+    return any(stride == 0 and size > 1 for stride, size in zip(t.stride(), t.shape))
+
+
 def _angles(cos, sin, batch: int, tokens: int, dim: int, dtype: torch.dtype):
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin must be given together")
@@ -115,10 +128,12 @@ class QuantizeKVPlan(AppendKVPlan):
             raise ValueError("positions must have the dtype of the lengths that are written")
         pos_dtype, num_positions = _positions(positions, batch, lengths_out)
         counts_dtype = _optional_counts(counts, batch, "counts")
-        if any(st == 0 and n > 1 for t in (cache.key, cache.value, cache.scales) for st, n in zip(t.stride(), t.shape)):
+        if any(_folded(t) for t in (cache.key, cache.value, cache.scales)) or cache.key.data_ptr() == cache.value.data_ptr():
             raise ValueError("the rows of a cache that is written must not share memory")
-        if lengths_out is not None and counts is not None and lengths_out.data_ptr() == counts.data_ptr():
+        if lengths_out is not None and counts is not None and _overlap(lengths_out, counts):
             raise ValueError("counts must not alias the lengths that are written")
+        if lengths_out is not None and lengths_out.data_ptr() != positions.data_ptr() and _overlap(lengths_out, positions):
+            raise ValueError("the lengths that are written may be the positions, but not a part of them")
         cos, sin, rope_strides = _angles(cos, sin, batch, tokens, dim, dtype)
         q_heads, qi, qo = 0, (0, 0, 0), (0, 0, 0)
         if query is None and query_out is not None:
@@ -133,6 +148,8 @@ class QuantizeKVPlan(AppendKVPlan):
                 raise ValueError("query / query_out must match the new rows in batch, tokens, head_dim and dtype")
             if query_out.data_ptr() == query.data_ptr():
                 raise ValueError("query_out must not alias query")
+            if _folded(query_out):
+                raise ValueError("the rows of query_out must not share memory")
             q_heads = shape[2]
         if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
             raise ValueError("status must be an int32 tensor")
@@ -214,6 +231,8 @@ class DequantizeKVPlan:
         counts_dtype = _optional_counts(counts, batch, "counts")
         if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
             raise ValueError("status must be an int32 tensor")
+        if _folded(key_out) or key_out.data_ptr() == value_out.data_ptr():
+            raise ValueError("the rows of key_out and value_out must not share memory")
         device = native.require_cuda(*cache.tensors(), key_out, value_out, starts, counts, status)
         desc = cache.descriptor()
         ptr = native._ptr

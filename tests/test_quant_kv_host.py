@@ -149,6 +149,28 @@ def test_aliased_lengths_and_missing_lengths_are_refused():
         sa.quantize_kv(contig(key=shared, value=shared), K, K)
 
 
+def test_overlapping_operands_are_refused():
+    codes = torch.zeros(2, 4, 16, 64, dtype=torch.int8)
+    with pytest.raises(ValueError, match="must not share memory"):
+        sa.quantize_kv(contig(key=codes, value=codes), K, K)
+    spread = torch.zeros(1, 3, 4, 64, dtype=torch.bfloat16).expand(2, 3, 4, 64)
+    with pytest.raises(ValueError, match="query_out must not share memory"):
+        sa.quantize_kv(contig(), K, K, query=K, query_out=spread)
+    with pytest.raises(ValueError, match="value_out must not share memory"):
+        sa.DequantizeKVPlan.build(contig(), spread, torch.zeros(1, 3, 4, 64, dtype=torch.bfloat16).expand(2, 3, 4, 64))
+    with pytest.raises(ValueError, match="value_out must not share memory"):
+        sa.DequantizeKVPlan.build(contig(), K, K)
+    buffer = torch.zeros(5, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not a part of them"):
+        sa.quantize_kv(contig(), K, K, positions=buffer[:2], lengths_out=buffer[1:3])
+    with pytest.raises(ValueError, match="counts must not alias"):
+        sa.quantize_kv(contig(), K, K, positions=buffer[:2], lengths_out=buffer[3:], counts=buffer[2:4])
+    with pytest.raises(RuntimeError, match="CUDA"):                       # beside each other, or the same, is fine
+        sa.quantize_kv(contig(), K, K, positions=buffer[:2], lengths_out=buffer[2:4])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        sa.quantize_kv(contig(), K, K, positions=buffer[:2], lengths_out=buffer[:2])
+
+
 @pytest.mark.parametrize("kwargs,match", [
     (dict(key_out=K.to(torch.int8)), "bf16, fp16 or fp32"),
     (dict(value_out=K.half()), "share a dtype"),
