@@ -19,20 +19,20 @@ int stream_kv_split(int group)
     return 0;
 }
 
-int stream_tile_tokens(int head_dim, bool quant) { return quant ? quant_tile_tokens(head_dim) : kTileBytes / (head_dim * 2); }
+int stream_tile_tokens(int head_dim, bool quant) { return quant ? kQuantTileTokens : kTileBytes / (head_dim * 2); }
 
 int stream_stages(int head_dim, bool rows16, bool quant) { return stages_of(head_dim, rows16, quant); }
 
 size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch, bool quant)
 {
-    const size_t warps = warps_of(head_dim, rows16, quant);
+    const size_t warps = kStreamWarps;
     const size_t bars = (warps * stages * 8 + 15) / 16 * 16;
     // Per-warp (o, m, l) areas plus (16-bit caches) the context-parallel staging rows (8-byte words).
     const size_t states = (warps + (quant ? 0 : 2)) * (rows16 ? 16 : 8) * (head_dim + 2) * 4;
     const size_t scratch = warps * 32 * 6 * 4;  // merges: 6 floats per thread
     // A stage: K and V tile, for 8-bit caches with the tile's scale bytes.
-    const size_t stage = quant ? static_cast<size_t>(quant_tile_tokens(head_dim)) * (2 * head_dim + 2) : 2 * kTileBytes;
-    const size_t floats = quant ? warps * quant_tile_tokens(head_dim) * 8 : 0;
+    const size_t stage = quant ? static_cast<size_t>(kQuantTileTokens) * (2 * head_dim + 2) : 2 * kTileBytes;
+    const size_t floats = quant ? warps * kQuantTileTokens * 8 : 0;
     return 1024 + warps * stages * stage + floats + bars + states + scratch + (2 * static_cast<size_t>(batch) + 1) * 4 + 16;
 }
 

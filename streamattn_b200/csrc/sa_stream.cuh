@@ -13,25 +13,18 @@ constexpr int kStreamWarps = SA_STREAM_WARPS;    // each with its own ring of ti
 #define SA_STREAM_STAGES 1
 #endif
 constexpr int kStreamStages = SA_STREAM_STAGES;  // 16 KB K+V tiles in flight per warp
-#ifndef SA_QW64
-#define SA_QW64 8
-#define SA_QT64 64
-#define SA_QS64 2
-#endif
-#ifndef SA_QW128
-#define SA_QW128 8
-#define SA_QT128 64
-#define SA_QS128 1
-#endif
-__host__ __device__ constexpr int quant_tile_tokens(int head_dim) { return head_dim == 64 ? SA_QT64 : SA_QT128; }  // 8-bit caches: 8 KB (D64) or 16 KB (D128) of codes a tile
 
-constexpr int warps_of(int head_dim, bool rows16, bool quant) { return !quant ? kStreamWarps : rows16 ? 8 : head_dim == 64 ? SA_QW64 : SA_QW128; }
+// 8-bit caches: tiles of 64 tokens, 8 KB of codes at D64 and 16 KB at D128, and 16 KB in flight a warp at either.
+// Tried at 8 rows x 2 KV heads x 65536 tokens, D64 (24.9 us, 27.5 in pages of 64): tiles of 128 tokens leave a
+// coarser last round; a third stage, or 10, 12 or 16 warps, spill or keep fewer bytes in flight - 12 warps gain 1-2 us in
+// pages and lose 2.7 on rows.
+constexpr int kQuantTileTokens = 64;
 
-// Tiles in flight per warp (the state areas of 16 head rows at D128 leave room for fewer).
+// Tiles in flight per warp.
 constexpr int stages_of(int head_dim, bool rows16, bool quant)
 {
-    if (quant) return rows16 ? 8192 / (quant_tile_tokens(head_dim) * head_dim) : head_dim == 64 ? SA_QS64 : SA_QS128;
-    return (head_dim == 128 && rows16 && kStreamStages > 2) ? 2 : kStreamStages;
+    if (quant) return 128 / head_dim;
+    return (head_dim == 128 && rows16 && kStreamStages > 2) ? 2 : kStreamStages;  // 16 rows' states leave room for fewer
 }
 
 constexpr int kCpMaxWorld = SA_CP_MAX_WORLD;

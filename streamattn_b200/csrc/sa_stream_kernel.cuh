@@ -15,7 +15,9 @@
 // The same kernel serves contiguous caches, paged caches (page-table lookup per
 // fragment) and seed-only decode (a short list of cache blocks); CODE != kCodeNone is
 // the form for 8-bit caches (codes and scale bytes, see sa_quant.cuh), which differs in
-// what a tile holds and in the arithmetic between a tile and the accumulators.
+// what a tile holds (64 tokens' codes and scale bytes), in how pages smaller than that arrive (16-byte copies
+// by the lanes), in the arithmetic between a tile and the accumulators (sa_stream_quant.cuh), in when
+// slices are cut at pair boundaries, and in that it has no dynamic schedule.
 //
 // Included by the files that instantiate it: sa_stream.cu (16-bit caches), sa_stream_e4m3.cu and
 // sa_stream_int8.cu.
@@ -615,7 +617,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 {
     constexpr bool QUANT = CODE != kCodeNone;
     constexpr bool PAGED = PLACE == kPlacePages || PLACE == kPlaceSmallPages;  // 8-bit caches only
-    constexpr int TILE_N = QUANT ? quant_tile_tokens(D) : kTileBytes / (D * 2);  // tokens per tile
+    constexpr int TILE_N = QUANT ? kQuantTileTokens : kTileBytes / (D * 2);  // tokens per tile
     constexpr int TILE_BYTES = QUANT ? TILE_N * D : kTileBytes;              // one K or one V tile
     constexpr int STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int SCALE_BYTES = QUANT ? TILE_N * 2 : 0;  // (K, V) scale bytes of a tile
@@ -1248,7 +1250,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 
         // Query fragments of this KV group (A operand of q.k), rows >= group are zero.
         uint32_t qa[KS_QK][4];
-        QuantWarp<T, D, QUANT ? TILE_N : 32, ROWS16, QUANT ? CODE : kCodeInt8> qw;  // 8-bit caches: all of the warp's arithmetic
+        QuantWarp<T, D, ROWS16, QUANT ? CODE : kCodeInt8> qw;  // 8-bit caches: all of the warp's arithmetic
         if constexpr (QUANT) {
             qw.begin(static_cast<const T *>(p.q) + b * p.q_sb + static_cast<int64_t>(kvh) * group * p.q_sh, p.q_sh, group,
                      p.scale_log2, g, t4);
@@ -1707,8 +1709,8 @@ cudaError_t launch_place(const CUtensorMap &mk, const CUtensorMap &mv, const Str
 {
     constexpr bool kQuant = CODE != kCodeNone;
     if (sp.group > 8)
-        return launch_instance<T, D, warps_of(D, true, kQuant), stages_of(D, true, kQuant), true, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
-    return launch_instance<T, D, warps_of(D, false, kQuant), stages_of(D, false, kQuant), false, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
+        return launch_instance<T, D, kStreamWarps, stages_of(D, true, kQuant), true, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
+    return launch_instance<T, D, kStreamWarps, stages_of(D, false, kQuant), false, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
 }
 
 template <typename T, int D, int CODE>

@@ -19,6 +19,15 @@
 // Every score is then multiplied by the token's K scale, 2^e exactly.  p is multiplied by the V scale
 // relative to a unit, 2^(e - v_exp + 15) <= 2^15 with v_exp the largest V byte so far: at the top of fp16's
 // range, where a small p or a small row of V keeps its eleven bits down to 2^-29 of the largest.
+//
+// What bounds it: at D128 memory (8 rows x 2 KV heads x 65536 tokens, 8 heads a group: 46 us for 271 MB, 5.85 TB/s;
+// 61 x 8 x 8192 int8: 164 us, 6.3 TB/s), at D64 the instructions between two tiles as much as memory
+// (24.9 us, 5.48 TB/s, of which 5 us are launch, first tile and merge).  Groups of 9 to 16 heads do the second
+// product twice per conversion and are bound by issue: 32 us at D64.  int8 costs 2.5 us more than e4m3 there: a byte
+// pair becomes two halves in five instructions against one.  What made the difference, at that D64 shape:
+// heads on M, tokens on N and one tile in four used 36.7 us; tokens on M (no padded rows) 33; e4m3 as fp16 instead
+// of e4m3 instructions 29.4; scales as floats once a token, places once a tile, the rescale skipped while the
+// maximum stands 27.2; instances by where the tokens lie 24.9.
 #pragma once
 
 #include <type_traits>
@@ -65,11 +74,6 @@ template <int OFFSET> __device__ __forceinline__ float2 lds_float2(uint32_t addr
 __device__ __forceinline__ void sts_float4(uint32_t addr, float a, float b, float c, float d)
 {
     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
-}
-
-__device__ __forceinline__ void sts_float2(uint32_t addr, float a, float b)
-{
-    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
 
 __device__ __forceinline__ void sts128_zero(uint32_t addr)
@@ -155,11 +159,10 @@ template <int D> __device__ __forceinline__ uint32_t piece(int row, int chunk)
     return row * D + ((D == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4);
 }
 
-template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp {
+template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
+    static constexpr int TILE_N = kQuantTileTokens;  // two tokens' scales a lane
     static constexpr int NH = ROWS16 ? 2 : 1;     // groups of eight heads
-    static constexpr int SUB = TILE_N < 64 ? TILE_N : 64;  // tokens whose scores are held at a time
-    static constexpr int MT = SUB / 16;           // ... in 16-token tiles
-    static constexpr int PER_LANE = TILE_N / 32;  // tokens whose scales a lane prepares
+    static constexpr int MT = TILE_N / 16;        // 16-token tiles
     static constexpr int KS = D / 32;             // k-steps of 32 dimensions
     static constexpr int DT = D / 16;             // output tiles
 
@@ -266,34 +269,16 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
 
         // The scale bytes become floats once a token: K's as it is, V's relative to the unit.  Tokens that are not
         // there get zeros, and so do their V codes: what the buffers hold for them is stale.
-        constexpr int WORDS = (PER_LANE + 1) / 2;
-        uint32_t pairs[WORDS];
-        if constexpr (PER_LANE == 4) {
-            const uint2 x = lds64<0>(sb + lane * 8);
-            pairs[0] = x.x;
-            pairs[WORDS - 1] = x.y;
-        } else if constexpr (PER_LANE == 2) {
-            pairs[0] = lds32<0>(sb + lane * 4);
-        } else {
-            pairs[0] = (lds32<0>(sb + (lane >> 1) * 4) >> ((lane & 1) * 16)) & 0xffffu;
-        }
+        uint32_t pairs = lds32<0>(sb + lane * 4);
         if (partial) {
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) {
-                if (!valid(PER_LANE * lane + 2 * i)) pairs[i] &= 0xffff0000u;
-                if (PER_LANE > 1 && !valid(PER_LANE * lane + 2 * i + 1)) pairs[i] &= 0x0000ffffu;
-            }
+            if (!valid(2 * lane)) pairs &= 0xffff0000u;
+            if (!valid(2 * lane + 1)) pairs &= 0x0000ffffu;
             for (int i = lane; i < TILE_N * (D / 16); i += 32)
                 if (!valid(i / (D / 16))) sts128_zero(vb + i * 16);
         }
-        uint32_t my_top = 0, nan_bytes = 0;
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            const uint32_t nan = __vcmpeq4(pairs[i], 0xffffffffu);
-            pairs[i] &= ~nan;
-            nan_bytes |= nan;
-            my_top = max(my_top, max((pairs[i] >> 8) & 0xffu, pairs[i] >> 24));
-        }
+        const uint32_t nan_bytes = __vcmpeq4(pairs, 0xffffffffu);
+        pairs &= ~nan_bytes;
+        const uint32_t my_top = max((pairs >> 8) & 0xffu, pairs >> 24);
         int top = static_cast<int>(__reduce_max_sync(0xffffffffu, nan_bytes != 0u ? 256u : my_top));
         if (top == 256) {
             has_nan = true;
@@ -302,16 +287,12 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
         const int old_exp = v_exp;
         v_exp = max(v_exp, top);
         const int off = (142 - v_exp) * (1 << 23);
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            const float k0 = __uint_as_float((pairs[i] << 23) & 0x7f800000u), k1 = __uint_as_float((pairs[i] << 7) & 0x7f800000u);
-            const float v0 = __int_as_float(max(static_cast<int>((pairs[i] << 15) & 0x7f800000u) + off, 0));
-            const float v1 = __int_as_float(max(static_cast<int>((pairs[i] >> 1) & 0x7f800000u) + off, 0));
-            if constexpr (PER_LANE > 1) sts_float4(fb + (PER_LANE * lane + 2 * i) * 8, k0, v0, k1, v1);
-            else sts_float2(fb + lane * 8, k0, v0);
-        }
+        sts_float4(fb + lane * 16, __uint_as_float((pairs << 23) & 0x7f800000u),
+                   __int_as_float(max(static_cast<int>((pairs << 15) & 0x7f800000u) + off, 0)),
+                   __uint_as_float((pairs << 7) & 0x7f800000u),
+                   __int_as_float(max(static_cast<int>((pairs >> 1) & 0x7f800000u) + off, 0)));
         __syncwarp();
-        float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);
+        const float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);
 
         // Every 16-token tile has the same swizzle, so a lane's places in it are computed once a tile.
         const int row_g = tile_token<D>(g);
@@ -328,150 +309,145 @@ template <typename T, int D, int TILE_N, bool ROWS16, int CODE> struct QuantWarp
             v_at[c] = vb + (D == 128 ? piece<D>(row, g) : piece<D>(row, g >> 1) + (g & 1) * 8);
         }
 
-#pragma unroll 1
-        for (int first = 0; first < TILE_N; first += SUB) {
-            if (first >= n_valid) break;
-            float s[MT][NH][4];
-            float v_weight[MT][2];
-            uint32_t k_from[KS];
+        float s[MT][NH][4];
+        float v_weight[MT][2];
+        uint32_t k_from[KS];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) k_from[ks] = kb + first * D + (k_at ^ (ks << 5));
-            unrolled<MT>([&](auto mt_c) {
-                constexpr int mt = decltype(mt_c)::value;
-                [[maybe_unused]] int hi[NH][4], lo[NH][4];
-                unrolled<KS>([&](auto ks_c) {
-                    constexpr int ks = decltype(ks_c)::value;
-                    uint32_t a[4];
-                    load_matrices<mt * 16 * D>(k_from[ks], a);
-                    if constexpr (CODE == kCodeE4M3) {
-                        uint32_t x[4], y[4];  // halves 0, 1 and 2, 3 of each word
+        for (int ks = 0; ks < KS; ++ks) k_from[ks] = kb + (k_at ^ (ks << 5));
+        unrolled<MT>([&](auto mt_c) {
+            constexpr int mt = decltype(mt_c)::value;
+            [[maybe_unused]] int hi[NH][4], lo[NH][4];
+            unrolled<KS>([&](auto ks_c) {
+                constexpr int ks = decltype(ks_c)::value;
+                uint32_t a[4];
+                load_matrices<mt * 16 * D>(k_from[ks], a);
+                if constexpr (CODE == kCodeE4M3) {
+                    uint32_t x[4], y[4];  // halves 0, 1 and 2, 3 of each word
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) decode4<CODE>(a[i], x[i], y[i]);
-#pragma unroll
-                        for (int nh = 0; nh < NH; ++nh) {
-                            mma_f16<ks == 0>(s[mt][nh], x[0], x[1], x[2], x[3], q[nh][ks][0], q[nh][ks][1]);
-                            mma_f16<false>(s[mt][nh], y[0], y[1], y[2], y[3], q[nh][ks][2], q[nh][ks][3]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int nh = 0; nh < NH; ++nh) {
-                            mma_int8<ks == 0>(hi[nh], a, q[nh][ks][0], q[nh][ks][1]);
-                            mma_int8<ks == 0>(lo[nh], a, q[nh][ks][2], q[nh][ks][3]);
-                        }
-                    }
-                });
-                const float2 kv0 = lds_float2<mt * 128>(f0 + first * 8), kv1 = lds_float2<mt * 128>(f1 + first * 8);
-                v_weight[mt][0] = kv0.y;
-                v_weight[mt][1] = kv1.y;
-#pragma unroll
-                for (int nh = 0; nh < NH; ++nh) {
-                    if constexpr (CODE == kCodeInt8) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)  // below 2^30 for D = 128
-                            s[mt][nh][e] = static_cast<float>(hi[nh][e] * 256 + lo[nh][e]);
-                    }
-                    s[mt][nh][0] *= kv0.x;
-                    s[mt][nh][1] *= kv0.x;
-                    s[mt][nh][2] *= kv1.x;
-                    s[mt][nh][3] *= kv1.x;
-                }
-            });
-            if (partial) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const bool ok0 = valid(first + mt * 16 + row_g), ok1 = valid(first + mt * 16 + (row_g ^ 1));
+                    for (int i = 0; i < 4; ++i) decode4<CODE>(a[i], x[i], y[i]);
 #pragma unroll
                     for (int nh = 0; nh < NH; ++nh) {
-                        if (!ok0) s[mt][nh][0] = s[mt][nh][1] = -INFINITY;
-                        if (!ok1) s[mt][nh][2] = s[mt][nh][3] = -INFINITY;
+                        mma_f16<ks == 0>(s[mt][nh], x[0], x[1], x[2], x[3], q[nh][ks][0], q[nh][ks][1]);
+                        mma_f16<false>(s[mt][nh], y[0], y[1], y[2], y[3], q[nh][ks][2], q[nh][ks][3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh) {
+                        mma_int8<ks == 0>(hi[nh], a, q[nh][ks][0], q[nh][ks][1]);
+                        mma_int8<ks == 0>(lo[nh], a, q[nh][ks][2], q[nh][ks][3]);
                     }
                 }
+            });
+            const float2 kv0 = lds_float2<mt * 128>(f0), kv1 = lds_float2<mt * 128>(f1);
+            v_weight[mt][0] = kv0.y;
+            v_weight[mt][1] = kv1.y;
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh) {
+                if constexpr (CODE == kCodeInt8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)  // below 2^30 for D = 128
+                        s[mt][nh][e] = static_cast<float>(hi[nh][e] * 256 + lo[nh][e]);
+                }
+                s[mt][nh][0] *= kv0.x;
+                s[mt][nh][1] *= kv0.x;
+                s[mt][nh][2] *= kv1.x;
+                s[mt][nh][3] *= kv1.x;
             }
+        });
+        if (partial) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const bool ok0 = valid(mt * 16 + row_g), ok1 = valid(mt * 16 + (row_g ^ 1));
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
+                    if (!ok0) s[mt][nh][0] = s[mt][nh][1] = -INFINITY;
+                    if (!ok1) s[mt][nh][2] = s[mt][nh][3] = -INFINITY;
+                }
+            }
+        }
 
-            // Online softmax.  The running maximum is subtracted before row_scale is applied, so that the largest p
-            // is exactly 1 however large the scores are (fma(s, scale, -max * scale) makes it 2^(rounding of the product)).
-            float sub[NH][2], alpha[NH][2];
-            bool same = unit == 1.0f;
+        // Online softmax.  The running maximum is subtracted before row_scale is applied, so that the largest p
+        // is exactly 1 however large the scores are (fma(s, scale, -max * scale) makes it 2^(rounding of the product)).
+        float sub[NH][2], alpha[NH][2];
+        bool same = unit == 1.0f;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float x = -INFINITY;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][nh][h], s[mt][nh][2 + h]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                same = same && !(x > m[nh][h]);
+                x = fmaxf(m[nh][h], x);
+                sub[nh][h] = x == -INFINITY ? 0.0f : x;
+                alpha[nh][h] = m[nh][h];
+                m[nh][h] = x;
+            }
+        }
+        if (!__all_sync(0xffffffffu, same)) {  // a new maximum or unit: after a row's first tiles rarely
 #pragma unroll
             for (int nh = 0; nh < NH; ++nh) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float x = -INFINITY;
+                    alpha[nh][h] = exp2f((alpha[nh][h] - sub[nh][h]) * row_scale[nh][h]);
+                    l[nh][h] *= alpha[nh][h];
+                    alpha[nh][h] *= unit;
+                }
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][nh][h], s[mt][nh][2 + h]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    same = same && !(x > m[nh][h]);
-                    x = fmaxf(m[nh][h], x);
-                    sub[nh][h] = x == -INFINITY ? 0.0f : x;
-                    alpha[nh][h] = m[nh][h];
-                    m[nh][h] = x;
+                for (int i = 0; i < DT; ++i) {
+                    o[nh][i][0] *= alpha[nh][0];
+                    o[nh][i][1] *= alpha[nh][1];
+                    o[nh][i][2] *= alpha[nh][0];
+                    o[nh][i][3] *= alpha[nh][1];
                 }
             }
-            if (!__all_sync(0xffffffffu, same)) {  // a new maximum or unit: after a row's first tiles rarely
-#pragma unroll
-                for (int nh = 0; nh < NH; ++nh) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        alpha[nh][h] = exp2f((alpha[nh][h] - sub[nh][h]) * row_scale[nh][h]);
-                        l[nh][h] *= alpha[nh][h];
-                        alpha[nh][h] *= unit;
-                    }
-#pragma unroll
-                    for (int i = 0; i < DT; ++i) {
-                        o[nh][i][0] *= alpha[nh][0];
-                        o[nh][i][1] *= alpha[nh][1];
-                        o[nh][i][2] *= alpha[nh][0];
-                        o[nh][i][3] *= alpha[nh][1];
-                    }
-                }
-                unit = 1.0f;
-            }
-
-            unrolled<MT>([&](auto mt_c) {
-                constexpr int mt = decltype(mt_c)::value;
-                const float v0 = v_weight[mt][0], v1 = v_weight[mt][1];
-                uint32_t b[NH][2];
-#pragma unroll
-                for (int nh = 0; nh < NH; ++nh) {
-                    const float p0 = exp2f((s[mt][nh][0] - sub[nh][0]) * row_scale[nh][0]);
-                    const float p1 = exp2f((s[mt][nh][1] - sub[nh][1]) * row_scale[nh][1]);
-                    const float p2 = exp2f((s[mt][nh][2] - sub[nh][0]) * row_scale[nh][0]);
-                    const float p3 = exp2f((s[mt][nh][3] - sub[nh][1]) * row_scale[nh][1]);
-                    l[nh][0] += p0 + p2;
-                    l[nh][1] += p1 + p3;
-                    b[nh][0] = transpose8(pack_halves(p0 * v0, p1 * v0));
-                    b[nh][1] = transpose8(pack_halves(p2 * v1, p3 * v1));
-                }
-                // The lane's D/8 bytes of its four tokens; two tokens are interleaved byte by byte, so that one
-                // conversion yields one operand register.  Byte 2 i is row g of output tile i, byte 2 i + 1 row g + 8.
-                uint32_t v[4][D / 32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if constexpr (D == 128) {
-                        const uint4 x = lds128<mt * 16 * D>(v_at[c] + first * D);
-                        v[c][0] = x.x; v[c][1] = x.y; v[c][2] = x.z; v[c][3] = x.w;
-                    } else {
-                        const uint2 x = lds64<mt * 16 * D>(v_at[c] + first * D);
-                        v[c][0] = x.x; v[c][1] = x.y;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    uint32_t a[2][4];
-                    decode4<CODE>(__byte_perm(v[0][i], v[1][i], 0x5140), a[0][0], a[0][1]);
-                    decode4<CODE>(__byte_perm(v[0][i], v[1][i], 0x7362), a[1][0], a[1][1]);
-                    decode4<CODE>(__byte_perm(v[2][i], v[3][i], 0x5140), a[0][2], a[0][3]);
-                    decode4<CODE>(__byte_perm(v[2][i], v[3][i], 0x7362), a[1][2], a[1][3]);
-#pragma unroll
-                    for (int nh = 0; nh < NH; ++nh) {
-                        mma_f16<false>(o[nh][2 * i], a[0][0], a[0][1], a[0][2], a[0][3], b[nh][0], b[nh][1]);
-                        mma_f16<false>(o[nh][2 * i + 1], a[1][0], a[1][1], a[1][2], a[1][3], b[nh][0], b[nh][1]);
-                    }
-                }
-            });
         }
+
+        unrolled<MT>([&](auto mt_c) {
+            constexpr int mt = decltype(mt_c)::value;
+            const float v0 = v_weight[mt][0], v1 = v_weight[mt][1];
+            uint32_t b[NH][2];
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh) {
+                const float p0 = exp2f((s[mt][nh][0] - sub[nh][0]) * row_scale[nh][0]);
+                const float p1 = exp2f((s[mt][nh][1] - sub[nh][1]) * row_scale[nh][1]);
+                const float p2 = exp2f((s[mt][nh][2] - sub[nh][0]) * row_scale[nh][0]);
+                const float p3 = exp2f((s[mt][nh][3] - sub[nh][1]) * row_scale[nh][1]);
+                l[nh][0] += p0 + p2;
+                l[nh][1] += p1 + p3;
+                b[nh][0] = transpose8(pack_halves(p0 * v0, p1 * v0));
+                b[nh][1] = transpose8(pack_halves(p2 * v1, p3 * v1));
+            }
+            // The lane's D/8 bytes of its four tokens; two tokens are interleaved byte by byte, so that one
+            // conversion yields one operand register.  Byte 2 i is row g of output tile i, byte 2 i + 1 row g + 8.
+            uint32_t v[4][D / 32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if constexpr (D == 128) {
+                    const uint4 x = lds128<mt * 16 * D>(v_at[c]);
+                    v[c][0] = x.x; v[c][1] = x.y; v[c][2] = x.z; v[c][3] = x.w;
+                } else {
+                    const uint2 x = lds64<mt * 16 * D>(v_at[c]);
+                    v[c][0] = x.x; v[c][1] = x.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                uint32_t a[2][4];
+                decode4<CODE>(__byte_perm(v[0][i], v[1][i], 0x5140), a[0][0], a[0][1]);
+                decode4<CODE>(__byte_perm(v[0][i], v[1][i], 0x7362), a[1][0], a[1][1]);
+                decode4<CODE>(__byte_perm(v[2][i], v[3][i], 0x5140), a[0][2], a[0][3]);
+                decode4<CODE>(__byte_perm(v[2][i], v[3][i], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) {
+                    mma_f16<false>(o[nh][2 * i], a[0][0], a[0][1], a[0][2], a[0][3], b[nh][0], b[nh][1]);
+                    mma_f16<false>(o[nh][2 * i + 1], a[1][0], a[1][1], a[1][2], a[1][3], b[nh][0], b[nh][1]);
+                }
+            }
+        });
     }
 
     // The warp's state into its area: rows of `stride` floats, (o[D], m, l), m in base-2 scores.

@@ -242,6 +242,48 @@ def test_row_subsets_states_and_page_walk(dev, kernel):
     assert bool(((o[:3] / l[:3, :, None] - want[:3, 0]).abs() <= tol[:3, 0]).all())
 
 
+@pytest.mark.parametrize("page,layout,dim,group", [(8, "HND", 64, 4), (32, "NHD", 128, 16), (64, "HND", 64, 12),
+                                                   (128, "NHD", 128, 24), (256, "HND", 128, 9), (0, "BNHD", 128, 20)])
+def test_wide_indices_subsets_and_walks_on_every_placement(dev, page, layout, dim, group):
+    """Lengths 0 and 1, row subsets, 64-bit tables and lengths, groups of more than 8 and 16 heads."""
+    B, H, lengths = 5, 2, [513, 0, 1, 320, 65]
+    kind = "paged" if page else "contig"
+    cache, mirror = filled(dev, kind, layout, "e4m3", B, H, dim, 768, lengths, page=page or 16, seed=page,
+                           table_dtype=torch.int64, lens_dtype=torch.int64)
+    q = new_rows((B, 1, H * group, dim), torch.bfloat16, 3).clamp(-30, 30)
+    out = torch.full((B, 1, H * group, dim), 5.0, dtype=torch.bfloat16, device=dev)
+    plan = sa.QuantDecodePlan.build(q.to(dev), cache, output=out, record_page_walk=bool(page))
+    assert plan.kernel_name == "sm100_tma_mma_stream"
+    plan.set_row_indices(torch.tensor([3, 1, 2], device=dev))
+    plan.run()
+    check(out, q, mirror, lengths, rows=[1, 2, 3])
+    assert bool((out[[0, 4]] == 5.0).all()) and not bool(out[1].any())
+    plan.set_row_indices(None)
+    plan.run()
+    check(out, q, mirror, lengths)
+    assert plan.device_status() == 0
+    if page:
+        walk = torch.full(tuple(mirror["table"].shape), -1, dtype=torch.int32)
+        for b, n in enumerate(lengths):
+            walk[b, :-(-n // page)] = mirror["table"][b, :-(-n // page)].int()
+        assert torch.equal(plan.trace.cpu(), walk)
+
+
+def test_a_large_batch_of_one_token_rows(dev):
+    """More rows than a CTA has threads, and more pairs than the grid has CTAs."""
+    B, H, D = 900, 2, 64
+    cache = sa.QuantPagedKVCache.empty(B, 16, H, D, batch=B, max_pages_per_request=3, device=dev)
+    cache.page_table[:, 0] = torch.randperm(B, generator=torch.Generator().manual_seed(1)).int().to(dev)
+    k, v = (torch.randn(B, 1, H, D, generator=torch.Generator(dev).manual_seed(i), device=dev).bfloat16() for i in (1, 2))
+    q = torch.randn(B, 1, 4 * H, D, device=dev).bfloat16()
+    moved = sa.quantize_kv(cache, k, v, query=q)
+    assert torch.equal(moved, q) and bool((cache.sequence_lengths == 1).all())
+    value = sa.dequantize_kv(cache, tokens=1, dtype=torch.float32)[1]
+    out = sa.stream_attn_quant_decode(q, cache).view(B, H, 4, D).float()
+    want = value[:, 0, :, None].expand_as(out)                            # a softmax of one token: its V row, rounded once
+    assert bool(((out - want).abs() <= want.abs() * 2 ** -8).all())
+
+
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_lengths_change_on_the_device_and_graphs_follow(dev, kernel):
     B, H, G, D = 2, 2, 4, 128
