@@ -741,6 +741,98 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     bool dyn_claims = false;                     // ... through the claim counter
     int dyn_chunk = 1;                           // tiles per claim
     int dyn_nw = 0, dyn_gw = 0;                  // warps working on the pair, this warp's index among them
+    // 8-bit caches: the smallest number of tiles, `level`, such that every pair can be split over CTAs that take at most
+    // that many each, whole CTAs to a pair, ceil(tiles / level) of them.  Equal slices would give total / C each, but a slice
+    // that crosses pairs costs its CTA a second segment, some 3 us, and with many pairs every CTA has one or two and most
+    // pairs are merged; so the CTAs are aligned while level is at most 2 + 8 pairs / C rounds of the warps above that (aligned and
+    // not: 128 pairs of 2048 tokens, D128, 14.2 and 18.7 us; 120 of 4096, D64, 16.6 and 19.0; 120 of 1024 to 8192, 25.5 and
+    // 29.6; 144 of 100 to 8192, 32 and 40; 48 of 30000 to 65536, D128, 105 and 99; 16 of 524288 170 and 166).
+    // Levels against slices rounded to pairs one after the other: 24 pairs of 16384 to 65536 29.5 -> 27.4 us, 32 of 8192 to
+    // 32768, int8, 25.5 -> 22.8.
+    auto align_quant = [&]() {
+        aligned = false;
+        if (total_tiles > 0 && num_pairs <= C) {
+            // CTAs of a pair.  A level's reciprocal is taken a little too small, so that this is never above the true ceiling.
+            auto ctas_of = [](int tiles, float inverse) -> int { return static_cast<int>(ceilf(static_cast<float>(tiles) * inverse)); };
+            auto inverse_of = [](int level) -> float { return 1.0f / static_cast<float>(level) * (1.0f - 0x1p-21f); };
+            auto row_tiles_of = [&](int b) -> int { return b < p.batch ? tiles_before(b + 1) - tiles_before(b) : 0; };
+            int level;
+            if (ragged) {
+                const int mine = row_tiles_of(lane);  // the first 32 rows stay in a register
+                int longest = mine;
+                for (int b = lane + 32; b < p.batch; b += 32) longest = max(longest, row_tiles_of(b));
+                longest = static_cast<int>(__reduce_max_sync(0xffffffffu, longest));
+                level = longest;  // one CTA a pair
+                int low = static_cast<int>(q_t) + (r_t != 0u);
+                if (longest > low + WARPS) {
+                    if (num_pairs < C) level = min(level, total_tiles / (C - num_pairs) + 1);  // the sum of the ceilings is at most C
+                    while (level - low > (low >> 5)) {
+                        const int mid = (low + level) >> 1;
+                        const float inverse = inverse_of(mid);
+                        int n = ctas_of(mine, inverse);
+                        for (int b = lane + 32; b < p.batch; b += 32) n += ctas_of(row_tiles_of(b), inverse);
+                        if (Hkv * static_cast<int>(__reduce_add_sync(0xffffffffu, n)) <= C) level = mid; else low = mid + 1;
+                    }
+                    if (longest <= level + WARPS) level = longest;  // a merge costs more than the round it would save
+                }
+            } else {
+                const int n = C / num_pairs;
+                level = (p.uniform_tiles + n - 1) / n;
+            }
+            aligned = static_cast<int64_t>(level) * C <= total_tiles + static_cast<int64_t>(WARPS) * (2 * C + 8 * num_pairs);
+            if (aligned) {
+                int first = 0, n = 0;  // first CTA of this CTA's row, CTAs of one of the row's pairs
+                int b = p.batch;
+                if (ragged) {
+                    const float inverse = inverse_of(level);
+                    for (int base = 0; base < p.batch && b == p.batch; base += 32) {
+                        const int mine = ctas_of(row_tiles_of(base + lane), inverse);
+                        int end = Hkv * mine;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const int y = __shfl_up_sync(0xffffffffu, end, o);
+                            if (lane >= o) end += y;
+                        }
+                        const unsigned hit = __ballot_sync(0xffffffffu, c < first + end);
+                        const int src = hit != 0u ? __ffs(hit) - 1 : 31;
+                        n = __shfl_sync(0xffffffffu, mine, src);
+                        first += __shfl_sync(0xffffffffu, end, src);
+                        if (hit != 0u) {
+                            b = base + src;
+                            first -= Hkv * n;
+                        }
+                    }
+                } else {
+                    n = (p.uniform_tiles + level - 1) / level;
+                    b = min(c / (Hkv * n), p.batch);
+                    first = b * Hkv * n;
+                }
+                if (b < p.batch) {
+                    const int h = (c - first) / n, k = c - first - h * n;
+                    const int tb = tiles_before(b), row_tiles = tiles_before(b + 1) - tb;
+                    al_pair = b * Hkv + h;
+                    al_first = c - k;
+                    al_nseg = n;
+                    al_start = Hkv * tb + h * row_tiles;
+                    al_end = al_start + row_tiles;
+                    if (p.schedule == kScheduleCyclic && row_tiles >= n * WARPS * (STAGES + 1)) {
+                        dyn = true;
+                        dyn_nw = n * WARPS;
+                        dyn_gw = k * WARPS + warp;
+                        lo = al_start;
+                        hi = al_end;
+                    } else {
+                        lo = al_start + static_cast<int>(static_cast<int64_t>(row_tiles) * k / n);
+                        hi = al_start + static_cast<int>(static_cast<int64_t>(row_tiles) * (k + 1) / n);
+                    }
+                }
+            }
+        }
+        if (!aligned) {
+            lo = range_lo(c);
+            hi = range_lo(c + 1);
+        }
+    };
     auto cut_tile_list = [&]() {
         total_tiles = Hkv * tiles_before(p.batch);
         q_t = static_cast<unsigned>(total_tiles) / static_cast<unsigned>(C);
@@ -752,15 +844,11 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         dyn = dyn_claims = false;
         dyn_chunk = 1;
         dyn_nw = dyn_gw = 0;
-        // 8-bit caches: a second segment costs a CTA about as much as a round of its warps' tiles (3 us).  With
-        // n = floor(C / pairs) CTAs for the pairs that get fewest, an aligned CTA takes C / (n pairs) times the T / (C WARPS)
-        // rounds of an equal slice; while that is at most 1.2 rounds more, the CTAs are aligned, and if a ragged pair's
-        // share comes out at none, every pair gets one (128 pairs of 512 tokens, D128: 10.6 -> 7.1 us, of 2048: 18.7 -> 14.2;
-        // 126 ragged ones of 132 to 526: 16.7 -> 9.7 us).
-        const int64_t fewest = num_pairs <= C ? static_cast<int64_t>(C / num_pairs) * num_pairs : 0;
-        const bool short_rows = QUANT && fewest > 0 &&
-                                static_cast<int64_t>(total_tiles) * 5 * (C - fewest) <= 6 * WARPS * C * fewest;
-        aligned = total_tiles > 0 && (4 * num_pairs <= C || short_rows) &&
+        if constexpr (QUANT) {
+            align_quant();
+            return;
+        }
+        aligned = total_tiles > 0 && 4 * num_pairs <= C &&
                   static_cast<uint64_t>(C) * static_cast<uint64_t>(total_tiles) < (1ull << 32);
         if (aligned) {
             // One pair per lane: lane pp computes cs(pp); cs(pp+1) comes from the neighbour lane.
@@ -824,7 +912,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 al_nseg = static_cast<int>(n_eff);
                 al_start = static_cast<int>(t0);
                 al_end = static_cast<int>(t1);
-                const bool claims = !QUANT && p.schedule == kScheduleClaims;
+                const bool claims = p.schedule == kScheduleClaims;
                 if ((claims || p.schedule == kScheduleCyclic) && n_eff == n_p && tiles_p >= n_p * WARPS * (STAGES + 1)) {
                     // Shared schedules: the pair's warps take tiles round-robin by position - all of
                     // them (cyclic), or only their first STAGES + 1, after which every tile is claimed
@@ -847,23 +935,6 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                         lo = static_cast<int>(t0 + static_cast<unsigned>(static_cast<uint64_t>(tiles_p) * k / n_eff));
                         hi = static_cast<int>(t0 + static_cast<unsigned>(static_cast<uint64_t>(tiles_p) * (k + 1) / n_eff));
                     }
-                }
-            }
-        }
-        if (QUANT && !aligned && short_rows && total_tiles > 0) {
-            int longest = 0;
-            for (int bb = lane; bb < p.batch; bb += 32) longest = max(longest, tiles_before(bb + 1) - tiles_before(bb));
-            if (__reduce_max_sync(0xffffffffu, longest) <= 4 * WARPS) {
-                aligned = true;
-                lo = hi = 0;
-                al_pair = -1;
-                if (c < num_pairs) {
-                    const int bb = c / Hkv, tb = tiles_before(bb), row_tiles = tiles_before(bb + 1) - tb;
-                    al_pair = c;
-                    al_first = c;
-                    al_nseg = 1;
-                    lo = al_start = Hkv * tb + (c - bb * Hkv) * row_tiles;
-                    hi = al_end = lo + row_tiles;
                 }
             }
         }
