@@ -56,7 +56,7 @@ enum sa_kernel_choice { SA_KERNEL_AUTO = 0, SA_KERNEL_STREAM = 1, SA_KERNEL_GENE
    faster on HBM-bound calls).  The split states are then grouped differently from launch to
    launch, so results agree within the float tolerance but are not bit-reproducible; without
    the flag every call with the same inputs returns the same bits.  Ignored where it does not
-   apply (generic kernel, fewer than four CTAs per pair, very long rows). */
+   apply (generic kernel, 8-bit caches, fewer than four CTAs per pair, very long rows). */
 #define SA_KERNEL_FLAG_DYNAMIC 0x100
 
 /* Bits of the device status word (sa_workspace_status). */

@@ -23,12 +23,12 @@ int stream_tile_tokens(int head_dim, bool quant) { return quant ? kQuantTileToke
 
 int stream_stages(int head_dim, bool rows16, bool quant) { return stages_of(head_dim, rows16, quant); }
 
-size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch, bool quant)
+size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch, bool quant, bool solo)
 {
     const size_t warps = kStreamWarps;
     const size_t bars = (warps * stages * 8 + 15) / 16 * 16;
     // Per-warp (o, m, l) areas plus (16-bit caches) the context-parallel staging rows (8-byte words).
-    const size_t states = (warps + (quant ? 0 : 2)) * (rows16 ? 16 : 8) * (head_dim + 2) * 4;
+    const size_t states = (solo ? 2 * warps : warps + (quant ? 0 : 2)) * (rows16 ? 16 : 8) * (head_dim + 2) * 4;
     const size_t scratch = warps * 32 * 6 * 4;  // merges: 6 floats per thread
     // A stage: K and V tile, for 8-bit caches with the tile's scale bytes.
     const size_t stage = quant ? static_cast<size_t>(kQuantTileTokens) * (2 * head_dim + 2) : 2 * kTileBytes;
@@ -66,6 +66,10 @@ cudaError_t launch_stream(const Problem &p, const StreamGeometry &geo, const CpF
     // A row subset makes the rows' tile counts differ (rows left out have none).
     sp.uniform_tiles = p.seq.num_rows >= 0 ? -1 : geo.uniform_tiles;
     sp.schedule = geo.schedule;
+    // More pairs than CTAs: slices cut by warps, which need room for two states a warp - up to 8 query heads a KV head, and at
+    // D128 up to some 2800 rows.
+    sp.solo = p.quant.code != kCodeNone && sp.group <= 8 && static_cast<int64_t>(p.batch) * sp.kv_heads > geo.num_ctas &&
+              stream_smem_bytes(p.head_dim, false, stages_of(p.head_dim, false, true), p.batch, true, true) <= kStreamSmemLimit;
     sp.wait_ns = p.wait_ns;
     sp.first_merges = geo.first_merges;
     sp.seq = p.seq;

@@ -68,7 +68,7 @@ struct StreamGeometry {
 int stream_kv_split(int group);
 int stream_tile_tokens(int head_dim, bool quant);
 int stream_stages(int head_dim, bool rows16, bool quant);
-size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch, bool quant);
+size_t stream_smem_bytes(int head_dim, bool rows16, int stages, int batch, bool quant, bool solo = false);
 constexpr size_t kStreamSmemLimit = 227 * 1024 - 64;
 
 // The instances over 8-bit caches, in translation units of their own.

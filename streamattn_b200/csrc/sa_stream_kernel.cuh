@@ -56,6 +56,7 @@ struct StreamParams {
     int tok_dim;         // TMA coordinate (1 or 2) that carries the token index
     int uniform_tiles;   // tiles per row when every row has the same length, else -1
     int schedule;        // kScheduleBlocked / kScheduleCyclic / kScheduleClaims
+    int solo;            // 8-bit caches: the instance whose warps take slices of their own
     int kv_split;        // virtual KV heads per physical KV head (kv_heads and group above are virtual)
     unsigned long long wait_ns;  // limit of every bounded wait
     int first_merges;    // the pair's first CTA merges its split states (no ticket): grids of at most one CTA per SM
@@ -610,7 +611,12 @@ struct Frag {
     int64_t trace_idx;  // slot of the page-walk trace to record, or -1
 };
 
-template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE>
+// SOLO (8-bit caches, more pairs than CTAs, so that every slice crosses pairs): each warp streams a part of the CTA's slice
+// by itself, without a barrier between pairs.  A pair that lies in one warp's part is finished by that warp; the others, one for
+// each border between parts at most, are combined by the whole CTA afterwards.  With a barrier a pair instead: 1024 pairs of 128
+// to 1024 tokens, D128, 94 us against 54; 256 of 128 to 2048 43 and 28; 488 of 512 to 2048, D64, 52 and 35; 488 of 2048 to 8192,
+// int8, D128, 121 and 111.  With fewer pairs the cut by warps gains nothing, and choosing at run time costs 1 us.
+template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE, bool SOLO>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                      const __grid_constant__ StreamParams p)
@@ -635,6 +641,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     constexpr int BAR_BYTES = (WARPS * STAGES * 8 + 15) / 16 * 16;
     constexpr int MERGE_ROWS = NTHREADS / (D / 4);  // head rows one merge pass covers
     constexpr int OWN = (ROWS * (D / 4) + NTHREADS - 1) / NTHREADS;  // work items per thread
+    static_assert(!SOLO || (QUANT && !ROWS16), "two states a warp");
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -642,7 +649,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     uint8_t *scale_floats = scale_ring + WARPS * STAGES * SCALE_BYTES;       // the scales of a warp's current tile as floats
     uint64_t *bars = reinterpret_cast<uint64_t *>(scale_floats + (QUANT ? WARPS * TILE_N * 8 : 0));
     float *states = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(bars) + BAR_BYTES);
-    uint64_t *cp_stage = reinterpret_cast<uint64_t *>(states + WARPS * STATE_FLOATS);  // context-parallel: rows to send
+    uint64_t *cp_stage = reinterpret_cast<uint64_t *>(states + (SOLO ? 2 : 1) * WARPS * STATE_FLOATS);  // context-parallel: rows to send
     float *scratch = reinterpret_cast<float *>(cp_stage + (QUANT ? 0 : STATE_FLOATS));  // merges: 6 floats per thread
     int *prefix = reinterpret_cast<int *>(scratch + NTHREADS * 6);         // ragged rows: tiles before row b
     int *vlens = prefix + p.batch + 1;                                     // ragged rows: length of row b (-1: not selected)
@@ -844,7 +851,11 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         dyn = dyn_claims = false;
         dyn_chunk = 1;
         dyn_nw = dyn_gw = 0;
-        if constexpr (QUANT) {
+        if constexpr (SOLO) {
+            lo = range_lo(c);
+            hi = range_lo(c + 1);
+            return;
+        } else if constexpr (QUANT) {
             align_quant();
             return;
         }
@@ -1036,8 +1047,12 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     // issued, so the counter's round trip overlaps a whole tile of work.
     // 8-bit caches: a tile holds half the bytes, so what is done once a tile weighs twice as much.  Their tiles
     // come in steps of a constant (there is no dynamic schedule), and positions are 32-bit integers.
-    int step_x = dyn ? al_start + dyn_gw : lo + warp;
-    const int step = dyn ? dyn_nw : WARPS, step_end = dyn ? al_end : hi;
+    auto part_lo = [&](int w) -> int {  // first tile of warp w's part (SOLO)
+        const int n = hi - lo;
+        return lo + (n / WARPS) * w + (n % WARPS) * w / WARPS;
+    };
+    int step_x = dyn ? al_start + dyn_gw : SOLO ? part_lo(warp) : lo + warp;
+    const int step = dyn ? dyn_nw : SOLO ? 1 : WARPS, step_end = dyn ? al_end : SOLO ? part_lo(warp + 1) : hi;
     auto next_tile = [&]() -> int {
         int x = -1;
         if constexpr (QUANT) {
@@ -1299,11 +1314,23 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         }
     }
 
-    int cur = lo;
+    int cur = lo, end = hi;
     int j = 0;          // next tile of this warp to consume
     bool dead = false;  // a bounded wait gave up: stop computing, keep the CTA barriers
+    bool parts = SOLO;  // the warps are streaming their parts
+    if (SOLO) {
+        cur = part_lo(warp);
+        end = step_end;
+    }
 
-    while (cur < hi) {
+    while (true) {
+        if (SOLO && parts && cur >= end) {
+            __syncthreads();
+            parts = false;
+            cur = lo;
+            end = hi;
+        }
+        if (cur >= end) break;
         // The segment: tiles [cur, seg_end) of one (row, kv head) pair.
         int b, kvh, row_tiles, pair_start;
         if (aligned) {
@@ -1315,9 +1342,47 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             locate(cur, b, kvh, row_tiles, pair_start);
         }
         const int pair_end = pair_start + row_tiles;
-        const int seg_end = hi < pair_end ? hi : pair_end;
+        const int seg_end = end < pair_end ? end : pair_end;
         const int pair = b * Hkv + kvh;
         const int64_t vlen = vlen_of(b);
+
+        const int64_t out_row0 = static_cast<int64_t>(b) * p.q_heads + static_cast<int64_t>(kvh) * group;
+        const bool cp_on = !QUANT && p.cp.world > 0;
+        auto store_result = [&](int row, int d4, const float4 &acc, float big, float total_l) {
+            if (p.out_mode == SA_OUT_FINAL) {
+                const float inv = total_l > 0.0f ? 1.0f / total_l : 0.0f;
+                T *dst = static_cast<T *>(p.out) + (out_row0 + row) * D + d4;
+                *reinterpret_cast<uint2 *>(dst) =
+                    make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
+            } else if (cp_on) {
+                // Context-parallel: the pair's state rows are staged in shared memory as tagged
+                // words; cp_broadcast_pair() then sends them to every rank's gather buffer with
+                // wide, lane-contiguous stores.
+                uint64_t *dst = cp_stage + row * STATE_STRIDE;
+                dst[d4] = cp_word(acc.x, p.cp.step);
+                dst[d4 + 1] = cp_word(acc.y, p.cp.step);
+                dst[d4 + 2] = cp_word(acc.z, p.cp.step);
+                dst[d4 + 3] = cp_word(acc.w, p.cp.step);
+                if (d4 == 0) {
+                    dst[D] = cp_word(big, p.cp.step);
+                    dst[D + 1] = cp_word(total_l, p.cp.step);
+                }
+            } else {
+                float *dst = static_cast<float *>(p.out) + (out_row0 + row) * STATE_STRIDE;
+                *reinterpret_cast<float2 *>(dst + d4) = make_float2(acc.x, acc.y);
+                *reinterpret_cast<float2 *>(dst + d4 + 2) = make_float2(acc.z, acc.w);
+                if (d4 == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(big, total_l);
+            }
+        };
+        if (SOLO && !parts) {
+            bool done = false;  // the pair lay in one warp's part
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) done = done || (part_lo(w) <= pair_start && pair_end <= part_lo(w + 1));
+            if (done) {
+                cur = seg_end;
+                continue;
+            }
+        } else {
 
         // Query fragments of this KV group (A operand of q.k), rows >= group are zero.
         uint32_t qa[KS_QK][4];
@@ -1544,7 +1609,23 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         SA_STAMP(3);
         // Warp state -> the warp's state area: [ROWS][D+2] floats = (o, m, l).
         if constexpr (QUANT) {
-            qw.store(states + warp * STATE_FLOATS, STATE_STRIDE, g, t4);
+            // Parts: the state of a pair that began before the part goes to the warp's first area, others to its second.
+            float *area = states + (SOLO ? 2 * warp + (cur > pair_start ? 0 : 1) : warp) * STATE_FLOATS;
+            qw.store(area, STATE_STRIDE, g, t4);
+            if (SOLO) {
+                if (cur == pair_start && seg_end == pair_end) {  // the whole pair
+                    __syncwarp();
+                    for (int item = lane; item < group * (D / 4); item += 32) {
+                        const int row = item / (D / 4), d4 = (item - row * (D / 4)) * 4;
+                        const float *from = area + row * STATE_STRIDE;
+                        const float2 a = *reinterpret_cast<const float2 *>(from + d4), b2 = *reinterpret_cast<const float2 *>(from + d4 + 2);
+                        store_result(row, d4, make_float4(a.x, a.y, b2.x, b2.y), from[D], from[D + 1]);
+                    }
+                    __syncwarp();
+                }
+                cur = seg_end;
+                continue;
+            }
         } else {
             l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], 1);
             l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], 2);
@@ -1572,6 +1653,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         }
         __syncthreads();
         SA_STAMP(4);
+        }
 
         // Combine the warps of this CTA, then either finish the pair or publish a state.
         // Work items are 4 consecutive columns of one head row.
@@ -1579,34 +1661,6 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         const int nseg = aligned ? al_nseg : owner(pair_end - 1) - first_cta + 1;
         const int64_t slot_stride = static_cast<int64_t>(group) * PART_STRIDE;
         float *my_slot = p.partials + (static_cast<int64_t>(c) + pair) * slot_stride;
-        const int64_t out_row0 = static_cast<int64_t>(b) * p.q_heads + static_cast<int64_t>(kvh) * group;
-        const bool cp_on = !QUANT && p.cp.world > 0;
-        auto store_result = [&](int row, int d4, const float4 &acc, float big, float total_l) {
-            if (p.out_mode == SA_OUT_FINAL) {
-                const float inv = total_l > 0.0f ? 1.0f / total_l : 0.0f;
-                T *dst = static_cast<T *>(p.out) + (out_row0 + row) * D + d4;
-                *reinterpret_cast<uint2 *>(dst) =
-                    make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
-            } else if (cp_on) {
-                // Context-parallel: the pair's state rows are staged in shared memory as tagged
-                // words; cp_broadcast_pair() then sends them to every rank's gather buffer with
-                // wide, lane-contiguous stores.
-                uint64_t *dst = cp_stage + row * STATE_STRIDE;
-                dst[d4] = cp_word(acc.x, p.cp.step);
-                dst[d4 + 1] = cp_word(acc.y, p.cp.step);
-                dst[d4 + 2] = cp_word(acc.z, p.cp.step);
-                dst[d4 + 3] = cp_word(acc.w, p.cp.step);
-                if (d4 == 0) {
-                    dst[D] = cp_word(big, p.cp.step);
-                    dst[D + 1] = cp_word(total_l, p.cp.step);
-                }
-            } else {
-                float *dst = static_cast<float *>(p.out) + (out_row0 + row) * STATE_STRIDE;
-                *reinterpret_cast<float2 *>(dst + d4) = make_float2(acc.x, acc.y);
-                *reinterpret_cast<float2 *>(dst + d4 + 2) = make_float2(acc.z, acc.w);
-                if (d4 == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(big, total_l);
-            }
-        };
         const int items = group * (D / 4);
         // The pair's ticket is taken now, before this CTA's state is even combined: it counts the
         // CTAs that have finished streaming and elects the last of them as the merger.  The
@@ -1624,6 +1678,14 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                          : "=r"(old_count)
                          : "l"(p.counters + pair)
                          : "memory");
+        // Where warp w's state of this segment is; null where its part holds none of it.
+        auto area_of = [&](int w) -> const float * {
+            if (!SOLO) return states + w * STATE_FLOATS;
+            const int first = part_lo(w), last = part_lo(w + 1);
+            if (first >= last || last <= cur || first >= seg_end) return nullptr;
+            return states + (2 * w + (first > pair_start ? 0 : 1)) * STATE_FLOATS;
+        };
+        float *parked = SOLO ? reinterpret_cast<float *>(ring) : states;  // the tiles have all been used then
         // The thread keeps the items it combined (OWN of them at most) and parks them in shared
         // memory once the warps' areas are free: if this CTA turns out to be the one that merges
         // the pair, its own state never has to come back from global memory.
@@ -1638,12 +1700,17 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const int d4 = (item - row * (D / 4)) * 4;
             float big = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) big = fmaxf(big, states[w * STATE_FLOATS + row * STATE_STRIDE + D]);
+            for (int w = 0; w < WARPS; ++w) {
+                const float *area = area_of(w);
+                if (!SOLO || area != nullptr) big = fmaxf(big, area[row * STATE_STRIDE + D]);
+            }
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float total_l = 0.0f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float *area = states + w * STATE_FLOATS + row * STATE_STRIDE;
+                const float *area = area_of(w);
+                if (SOLO && area == nullptr) continue;
+                area += row * STATE_STRIDE;
                 const float wgt = exp2_diff(area[D], big);
                 const float2 lo2 = *reinterpret_cast<const float2 *>(area + d4);
                 const float2 hi2 = *reinterpret_cast<const float2 *>(area + d4 + 2);
@@ -1675,7 +1742,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             for (int k = 0; k < OWN; ++k) {
                 const int item = tid + k * NTHREADS;
                 if (item < items) {
-                    float *dst = states + item * 6;
+                    float *dst = parked + item * 6;
                     *reinterpret_cast<float2 *>(dst) = make_float2(own[k][0], own[k][1]);
                     *reinterpret_cast<float2 *>(dst + 2) = make_float2(own[k][2], own[k][3]);
                     *reinterpret_cast<float2 *>(dst + 4) = make_float2(own[k][4], own[k][5]);
@@ -1699,7 +1766,7 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     const int per_thread = static_cast<int>(
                         (static_cast<float>(nseg + sharers - 1) + 0.5f) * __frcp_rn(static_cast<float>(sharers)));
                     float *slots = first_slot + r0 * PART_STRIDE;
-                    const float *mine = states + k * NTHREADS * 6;
+                    const float *mine = parked + k * NTHREADS * 6;
                     if (per_thread <= 3)
                         merge_pair_states<D, NTHREADS, 3>(slots, slot_stride, nseg, c - first_cta, mine,
                                                                   sub_items, scratch, tid, p.wait_ns, p.status);
@@ -1739,12 +1806,12 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     }
 }
 
-template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE>
+template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE, bool SOLO>
 cudaError_t launch_instance(const CUtensorMap &mk, const CUtensorMap &mv, const StreamParams &sp, int ctas,
                             int batch, cudaStream_t stream)
 {
-    auto kernel = stream_decode_kernel<T, D, WARPS, STAGES, ROWS16, CODE, PLACE>;
-    const size_t smem = stream_smem_bytes(D, ROWS16, STAGES, batch, CODE != kCodeNone);
+    auto kernel = stream_decode_kernel<T, D, WARPS, STAGES, ROWS16, CODE, PLACE, SOLO>;
+    const size_t smem = stream_smem_bytes(D, ROWS16, STAGES, batch, CODE != kCodeNone, SOLO);
     // Opt in to the dynamic shared memory this launch needs (grows only; per device).
     static std::mutex mu;
     static size_t configured[64] = {};
@@ -1780,8 +1847,12 @@ cudaError_t launch_place(const CUtensorMap &mk, const CUtensorMap &mv, const Str
 {
     constexpr bool kQuant = CODE != kCodeNone;
     if (sp.group > 8)
-        return launch_instance<T, D, kStreamWarps, stages_of(D, true, kQuant), true, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
-    return launch_instance<T, D, kStreamWarps, stages_of(D, false, kQuant), false, CODE, PLACE>(mk, mv, sp, ctas, sp.batch, stream);
+        return launch_instance<T, D, kStreamWarps, stages_of(D, true, kQuant), true, CODE, PLACE, false>(mk, mv, sp, ctas, sp.batch, stream);
+    if constexpr (kQuant) {
+        if (sp.solo)
+            return launch_instance<T, D, kStreamWarps, stages_of(D, false, kQuant), false, CODE, PLACE, true>(mk, mv, sp, ctas, sp.batch, stream);
+    }
+    return launch_instance<T, D, kStreamWarps, stages_of(D, false, kQuant), false, CODE, PLACE, false>(mk, mv, sp, ctas, sp.batch, stream);
 }
 
 template <typename T, int D, int CODE>

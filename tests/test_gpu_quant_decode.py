@@ -370,6 +370,48 @@ def test_many_short_rows(dev, batch, heads, capacity, low, page):
         assert bool(((got - want).abs() <= tol).all()), (splits, float(((got - want).abs() - tol).max()))
 
 
+@pytest.mark.parametrize("code,dtype,dim,batch,heads,group,capacity,low", [
+    (torch.int8, torch.float16, 128, 30, 8, 4, 1024, 0), (torch.float8_e4m3fn, torch.bfloat16, 64, 3, 60, 8, 4096, 3000),
+    (torch.float8_e4m3fn, torch.float16, 128, 21, 9, 1, 640, 1), (torch.int8, torch.bfloat16, 64, 50, 4, 12, 512, 0)])
+@pytest.mark.parametrize("page", [0, 8, 64])
+def test_more_pairs_than_ctas(dev, code, dtype, dim, batch, heads, group, capacity, low, page):
+    """Slices that hold pairs, end in them and lie inside them; outputs and states; a subset of the rows."""
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(low, capacity + 1, (batch,), generator=g)
+    lengths[batch // 2] = capacity
+    k, v = (torch.randn(batch, capacity, heads, dim, generator=g).to(dtype).to(dev) for _ in range(2))
+    q = torch.randn(batch, 1, heads * group, dim, generator=g).to(dtype).to(dev)
+    if page:
+        cache = sa.QuantPagedKVCache.empty(batch * capacity // page, page, heads, dim, batch=batch, dtype=code, layout="NHD",
+                                           max_pages_per_request=capacity // page, device=dev)
+        cache.page_table.copy_(torch.randperm(batch * capacity // page, generator=g).view(batch, -1))
+    else:
+        cache = sa.QuantKVCache.empty(batch, heads, capacity, dim, device=dev, dtype=code)
+    sa.quantize_kv(cache, k, v, counts=lengths.to(dev))
+    key, value = (x.transpose(1, 2).double() for x in sa.dequantize_kv(cache, dtype=torch.float32))
+    qh = q[:, 0].double().view(batch, heads, group, dim)
+    mask = torch.arange(capacity, device=dev)[None, None, None] >= lengths.to(dev)[:, None, None, None]
+    p = torch.softmax((qh @ key.transpose(2, 3) / dim ** 0.5).masked_fill(mask, -1e300), -1).masked_fill(mask, 0.0)
+    want, spread = p @ value, p @ value.abs()
+    reach = (qh.abs() @ key.abs().transpose(2, 3)).masked_fill(mask, 0.0).amax(-1, keepdim=True) / dim ** 0.5
+    plan = sa.QuantDecodePlan.build(q, cache)
+    got = plan.run().double().view_as(want)
+    tol = tolerance(want, spread, reach, dtype, dim, capacity)
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() - tol).max())
+    first = plan.output.clone()
+    assert torch.equal(plan.run(), first) and plan.device_status() == 0
+    plan.output.fill_(5.0)
+    rows = torch.arange(0, batch, 2, device=dev)
+    plan.set_row_indices(rows)
+    got = plan.run().double().view_as(want)
+    assert bool(((got - want).abs() <= tol)[rows].all()) and bool((got[1::2] == 5.0).all())
+    state = sa.QuantDecodePlan.build(q, cache, return_state=True).run().double().view(batch, heads, group, dim + 2)
+    some = (lengths > 0).to(dev)
+    tol = tolerance(want, spread, reach, torch.float32, dim, capacity)
+    assert bool(((state[..., :dim] / state[..., dim + 1:] - want).abs() <= tol)[some].all())
+    assert bool((state[~some][..., dim + 1] == 0).all()) and bool(torch.isinf(state[~some][..., dim]).all())
+
+
 def test_strided_query_and_views_of_larger_caches(dev):
     B, H, G, D, lengths = 2, 2, 4, 64, [90, 33]
     cache, mirror = filled(dev, "contig", "BHND", "e4m3", B, H, D, 96, lengths, seed=7)
