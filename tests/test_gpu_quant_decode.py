@@ -269,9 +269,9 @@ def test_wide_indices_subsets_and_walks_on_every_placement(dev, page, layout, di
         assert torch.equal(plan.trace.cpu(), walk)
 
 
-def test_a_large_batch_of_one_token_rows(dev):
+@pytest.mark.parametrize("B,H,D", [(900, 2, 64), (3500, 1, 128)], ids=["warps' slices", "no room for them"])
+def test_a_large_batch_of_one_token_rows(dev, B, H, D):
     """More rows than a CTA has threads, and more pairs than the grid has CTAs."""
-    B, H, D = 900, 2, 64
     cache = sa.QuantPagedKVCache.empty(B, 16, H, D, batch=B, max_pages_per_request=3, device=dev)
     cache.page_table[:, 0] = torch.randperm(B, generator=torch.Generator().manual_seed(1)).int().to(dev)
     k, v = (torch.randn(B, 1, H, D, generator=torch.Generator(dev).manual_seed(i), device=dev).bfloat16() for i in (1, 2))
