@@ -9,11 +9,11 @@
 // such accesses (D no multiple of 16, odd strides) take one warp a unit with single-element accesses.
 //
 // Measured (bytes as above against the time): 8 x 4096 tokens x 2 heads, D64, bf16 with rotation and 16 query heads to
-// e4m3 33.8 us, 5.0 TB/s; 13 ragged rows of up to 8190 tokens x 8 heads, D128, fp16 to int8 in token-major pages 88 us,
+// e4m3 32.1 us, 5.2 TB/s; 13 ragged rows of up to 8190 tokens x 8 heads, D128, fp16 to int8 in token-major pages 88 us,
 // 4.9 TB/s; read back: ragged 8 x 65536 x 2, D64, pages of 16 46 us, 5.9 TB/s; 3 x 32768 x 8, D128, int8 to fp16 91 us,
 // 6.6 TB/s.  One token a row (8 rows, 2 + 16 heads): 6.0 us, the launch and one chain of position, page id and rows.
 // What made the difference: pieces of both halves of a row in one lane, so that rotation needs no other lane and each
-// unit costs half the index arithmetic (write 190 -> 91 us, 66 -> 33.5; read 113 -> 91, 59 -> 44).  Putting the
+// unit costs half the index arithmetic (write 190 -> 91 us, 66 -> 33; read 113 -> 91, 59 -> 44).  Putting the
 // page id's look-up behind the row loads gained nothing.
 #include <algorithm>
 
@@ -208,8 +208,10 @@ template <typename T> struct Halves {
     }
 };
 
+// 16-bit rows: registers for five CTAs an SM with rotation (48; 64 and four without the bound: 33.2 -> 32.1 us for the chunk
+// above), for six without (40; five: 91.2 -> 88.8 us for the prompts).
 template <typename T, int CODE, bool ROPE>
-__global__ void __launch_bounds__(kThreads) quantize_vector_kernel(const __grid_constant__ QuantizeParams p, int lane_shift)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (ROPE ? 5 : 6) : 1) quantize_vector_kernel(const __grid_constant__ QuantizeParams p, int lane_shift)
 {
     wait_for_stream();
     const int b = blockIdx.y;
