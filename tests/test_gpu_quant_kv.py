@@ -302,6 +302,36 @@ def test_update_replays_in_a_graph_and_runs_on_other_streams(dev):
     assert cache.sequence_lengths.tolist() == [20] * B
 
 
+@pytest.mark.parametrize("batch,tokens,heads,dim,page", [(5000, 40, 2, 64, 16), (9, 5000, 8, 128, 64), (6, 8191, 4, 64, 8)])
+@pytest.mark.parametrize("new_layout", ["BNHD", "BHND"])
+def test_large_ragged_writes_give_the_bytes_of_even_ones(dev, batch, tokens, heads, dim, page, new_layout):
+    """Threads that take several units: same bytes, nothing behind the counts, bad pages and lengths as ever."""
+    g = torch.Generator(dev).manual_seed(batch)
+    pages = -(-tokens // page)
+    shape = (batch, tokens, heads, dim) if new_layout == "BNHD" else (batch, heads, tokens, dim)
+    k, v, cos, sin = (torch.randn(s, generator=g, device=dev).bfloat16() for s in (shape, shape, (1, tokens, dim), (1, tokens, dim)))
+    counts = torch.randint(0, tokens + 1, (batch,), generator=g, device=dev)
+    counts[:2] = tokens
+    even, ragged = (sa.QuantPagedKVCache.empty(batch * pages, page, heads, dim, batch=batch, max_pages_per_request=pages, device=dev)
+                    for _ in range(2))
+    for cache in (even, ragged):
+        cache.page_table.copy_(torch.arange(batch * pages, device=dev).view(batch, pages))
+    ragged.page_table[1, 0] = -1                                          # its first tokens have no page, the others do
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    sa.quantize_kv(even, k, v, cos=cos, sin=sin, new_layout=new_layout)
+    sa.quantize_kv(ragged, k, v, cos=cos, sin=sin, new_layout=new_layout, counts=counts, status=status)
+    assert int(status) == native.SA_DEV_BAD_PAGE and bool((even.sequence_lengths == tokens).all())
+    want = counts.clone()
+    want[1] = 0
+    assert torch.equal(ragged.sequence_lengths.long(), want)
+    written = torch.arange(pages * page, device=dev)[None] < counts[:, None]
+    written[1, :page] = False
+    written = written.view(batch * pages, 1, page, 1)
+    for name in ("key", "value", "scales"):
+        a, b = (getattr(c, name).view(torch.uint8) for c in (even, ragged))
+        assert torch.equal(torch.where(written, a, torch.zeros_like(a)), b)
+
+
 def test_many_ctas_advance_their_row_in_place_once(dev):
     """Lengths that are positions too: no CTA of a row may see the new value."""
     B, T, H, D = 5, 700, 4, 128
