@@ -5,16 +5,17 @@
 //   S^T[token, head] = K q^T          tokens on the M rows of the tensor-core instructions, heads on N
 //   O^T[dim, head]  += V^T P^T
 //
-// e4m3   q is multiplied by the power of two that brings its largest element to [2^14, 2^15) and becomes fp16:
-//        exact for all but elements some 2^30 times smaller than that one.  The codes of K are converted to fp16, in
-//        which they are exact, and the products accumulate in fp32.  (There is an instruction with e4m3
-//        operands, but on this GPU it executes as conversions and fp16 products: measured 10 instructions
-//        and 16 cycles of the tensor pipe for its 16 x 8 x 32, where two fp16 instructions take the same.)
-// int8   the 8-bit integer instruction is native and twice as fast as fp16, so the codes of K go from shared
-//        memory into it as they are: q is scaled to integers of at most 32512 = 127 * 256 and split into two bytes,
-//        hi * 256 + lo, off by 2^-17 of the row's largest element; products and sums are exact in int32.
-// P V uses fp16 for both: p has a far larger range than two bytes hold (the tail of a long row may carry all of
-// its weight at 2^-20 of the maximum a token), and the codes are exact in fp16.
+// q is multiplied by the power of two that brings its largest element to [2^14, 2^15) and becomes fp16: exact for
+// all but elements some 2^30 times smaller than that one.  The codes of K and of V are converted to fp16, in which
+// either type of them is exact, and the products accumulate in fp32.
+// e4m3   There is an instruction with e4m3 operands, but on this GPU it executes as conversions and fp16 products:
+//        measured 10 instructions and 16 cycles of the tensor pipe for its 16 x 8 x 32, where two fp16
+//        instructions take the same.
+// int8   The 8-bit integer instruction is native and needs no conversion of K, but it wants the query in bytes: two of
+//        them hold every element to a step of 2^-16 of the largest, which loses the small elements of a
+//        query that has a few large ones, however small the K channels under those are.
+// P V uses fp16 for p too: it has a far larger range than two bytes hold (the tail of a long row may carry all of
+// its weight at 2^-20 of the maximum a token).
 //
 // Every score is then multiplied by the token's K scale, 2^e exactly.  p is multiplied by the V scale
 // relative to a unit, 2^(e - v_exp + 15) <= 2^15 with v_exp the largest V byte so far: at the top of fp16's
@@ -81,21 +82,6 @@ __device__ __forceinline__ void sts128_zero(uint32_t addr)
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
 }
 
-// FIRST: c is the product alone, not added to.
-template <bool FIRST> __device__ __forceinline__ void mma_int8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    if constexpr (FIRST)
-        asm volatile(
-            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // f(std::integral_constant<int, 0>) ... f(std::integral_constant<int, N - 1>): an unrolled loop whose index
 // is a constant expression.
 template <int N, typename F, int... I> __device__ __forceinline__ void unrolled(F &&f, std::integer_sequence<int, I...>)
@@ -107,6 +93,7 @@ template <int N, typename F> __device__ __forceinline__ void unrolled(F &&f)
     unrolled<N>(static_cast<F &&>(f), std::make_integer_sequence<int, N>{});
 }
 
+// FIRST: c is the product alone, not added to.
 template <bool FIRST>
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -166,7 +153,7 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
     static constexpr int KS = D / 32;             // k-steps of 32 dimensions
     static constexpr int DT = D / 16;             // output tiles
 
-    // Operand registers of a k-step.  e4m3: two of each of its two fp16 instructions; int8: two of the high, two of the low bytes.
+    // Operand registers of a k-step: two of each of its two instructions.
     uint32_t q[NH][KS][4];
     float row_scale[NH][2];      // heads 2 t4 and 2 t4 + 1: what turns the products into base-2 scores
     float m[NH][2], l[NH][2];    // running maximum (in the products' unit) and this lane's part of the sum
@@ -210,39 +197,18 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
             }
-            float scale;
-            if constexpr (CODE == kCodeE4M3) {
-                // Exponent of the factor: at least -113, and at most 100 to keep the scale clear of zero.
-                const int up = amax == 0 ? 0 : min(14 + 127 - static_cast<int>(amax >> 23), 100);
-                const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-                scale = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-                // A 32-bit word of K codes c0 .. c3 becomes the halves c0 c1 and c2 c3; a lane's word 4 t4 .. of the first
-                // 16 bytes of a k-step meets the lane's word of the second 16 bytes in one instruction each.
+            // Exponent of the factor: at least -113, and at most 100 to keep the scale clear of zero.
+            const int up = amax == 0 ? 0 : min(14 + 127 - static_cast<int>(amax >> 23), 100);
+            const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+            const float scale = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            // A 32-bit word of K codes c0 .. c3 becomes the halves c0 c1 and c2 c3; a lane's word 4 t4 .. of the first
+            // 16 bytes of a k-step meets the lane's word of the second 16 bytes in one instruction each.
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    q[nh][ks][0] = pack_halves(x[ks][0] * factor, x[ks][1] * factor);
-                    q[nh][ks][1] = pack_halves(x[ks][4] * factor, x[ks][5] * factor);
-                    q[nh][ks][2] = pack_halves(x[ks][2] * factor, x[ks][3] * factor);
-                    q[nh][ks][3] = pack_halves(x[ks][6] * factor, x[ks][7] * factor);
-                }
-            } else {
-                const float big = fmaxf(__uint_as_float(amax), __uint_as_float(27u << 23));
-                const float inv = 32512.0f / big;
-                scale = scale_log2 * (big * (1.0f / 32512.0f));
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        int hi[4], lo[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int v = max(min(__float2int_rn(x[ks][half * 4 + i] * inv), 32512), -32512);
-                            hi[i] = (v + 128) >> 8;
-                            lo[i] = v - hi[i] * 256;
-                        }
-                        q[nh][ks][half] = bytes4(hi);
-                        q[nh][ks][2 + half] = bytes4(lo);
-                    }
+            for (int ks = 0; ks < KS; ++ks) {
+                q[nh][ks][0] = pack_halves(x[ks][0] * factor, x[ks][1] * factor);
+                q[nh][ks][1] = pack_halves(x[ks][4] * factor, x[ks][5] * factor);
+                q[nh][ks][2] = pack_halves(x[ks][2] * factor, x[ks][3] * factor);
+                q[nh][ks][3] = pack_halves(x[ks][6] * factor, x[ks][7] * factor);
             }
             row_scale[nh][0] = __shfl_sync(0xffffffffu, scale, 8 * t4);
             row_scale[nh][1] = __shfl_sync(0xffffffffu, scale, 8 * t4 + 4);
@@ -252,11 +218,6 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.0f;
         }
-    }
-
-    __device__ __forceinline__ static uint32_t bytes4(const int (&v)[4])
-    {
-        return __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
     }
 
     // One tile: codes at kb and vb, scale pairs at sb, room for TILE_N float pairs at fb (shared memory).
@@ -316,26 +277,17 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
         for (int ks = 0; ks < KS; ++ks) k_from[ks] = kb + (k_at ^ (ks << 5));
         unrolled<MT>([&](auto mt_c) {
             constexpr int mt = decltype(mt_c)::value;
-            [[maybe_unused]] int hi[NH][4], lo[NH][4];
             unrolled<KS>([&](auto ks_c) {
                 constexpr int ks = decltype(ks_c)::value;
                 uint32_t a[4];
                 load_matrices<mt * 16 * D>(k_from[ks], a);
-                if constexpr (CODE == kCodeE4M3) {
-                    uint32_t x[4], y[4];  // halves 0, 1 and 2, 3 of each word
+                uint32_t x[4], y[4];  // halves 0, 1 and 2, 3 of each word
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) decode4<CODE>(a[i], x[i], y[i]);
+                for (int i = 0; i < 4; ++i) decode4<CODE>(a[i], x[i], y[i]);
 #pragma unroll
-                    for (int nh = 0; nh < NH; ++nh) {
-                        mma_f16<ks == 0>(s[mt][nh], x[0], x[1], x[2], x[3], q[nh][ks][0], q[nh][ks][1]);
-                        mma_f16<false>(s[mt][nh], y[0], y[1], y[2], y[3], q[nh][ks][2], q[nh][ks][3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int nh = 0; nh < NH; ++nh) {
-                        mma_int8<ks == 0>(hi[nh], a, q[nh][ks][0], q[nh][ks][1]);
-                        mma_int8<ks == 0>(lo[nh], a, q[nh][ks][2], q[nh][ks][3]);
-                    }
+                for (int nh = 0; nh < NH; ++nh) {
+                    mma_f16<ks == 0>(s[mt][nh], x[0], x[1], x[2], x[3], q[nh][ks][0], q[nh][ks][1]);
+                    mma_f16<false>(s[mt][nh], y[0], y[1], y[2], y[3], q[nh][ks][2], q[nh][ks][3]);
                 }
             });
             const float2 kv0 = lds_float2<mt * 128>(f0), kv1 = lds_float2<mt * 128>(f1);
@@ -343,11 +295,6 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
             v_weight[mt][1] = kv1.y;
 #pragma unroll
             for (int nh = 0; nh < NH; ++nh) {
-                if constexpr (CODE == kCodeInt8) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)  // below 2^30 for D = 128
-                        s[mt][nh][e] = static_cast<float>(hi[nh][e] * 256 + lo[nh][e]);
-                }
                 s[mt][nh][0] *= kv0.x;
                 s[mt][nh][1] *= kv0.x;
                 s[mt][nh][2] *= kv1.x;
