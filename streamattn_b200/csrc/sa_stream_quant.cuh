@@ -17,7 +17,9 @@
 // P V uses fp16 for p too: it has a far larger range than two bytes hold (the tail of a long row may carry all of
 // its weight at 2^-20 of the maximum a token).
 //
-// Every score is then multiplied by the token's K scale, 2^e exactly.  p is multiplied by the V scale
+// Every score is then multiplied by the token's K scale, 2^(e - 127 - k_down) exactly, and row_scale puts the powers
+// of two right that the query took and k_down left out.  The products are below 2^31, the codes times their scale below
+// 2^128, so scores at 2^-24 (k_down = 24) of the products stay finite for every finite K.  p is multiplied by the V scale
 // relative to a unit, 2^(e - v_exp + 15) <= 2^15 with v_exp the largest V byte so far: at the top of fp16's
 // range, where a small p or a small row of V keeps its eleven bits down to 2^-29 of the largest.
 //
@@ -155,6 +157,7 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
 
     // Operand registers of a k-step: two of each of its two instructions.
     uint32_t q[NH][KS][4];
+    int k_down;                  // (warp) powers of two left out of the K scales, as the exponent field of a float
     float row_scale[NH][2];      // heads 2 t4 and 2 t4 + 1: what turns the products into base-2 scores
     float m[NH][2], l[NH][2];    // running maximum (in the products' unit) and this lane's part of the sum
     float o[NH][DT][4];          // in units of 2^(v_exp - 142)
@@ -168,6 +171,7 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
         v_exp = 16;
         has_nan = false;
         nan_heads = 0;
+        int up[NH];  // exponent of the factor of head g of each eight, in [-113, 140]
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
             const bool ok = nh * 8 + g < group;
@@ -197,26 +201,40 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
             }
-            // Exponent of the factor: at least -113, and at most 100 to keep the scale clear of zero.
-            const int up = amax == 0 ? 0 : min(14 + 127 - static_cast<int>(amax >> 23), 100);
-            const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-            const float scale = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            up[nh] = amax < (1u << 23) ? 0 : 14 + 127 - static_cast<int>(amax >> 23);  // (subnormal numbers count as zeros)
+            const int up_half = up[nh] / 2;  // the factor in two steps: as one it might pass fp32's range
+            const float f0 = __uint_as_float(static_cast<uint32_t>(127 + up_half) << 23);
+            const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up[nh] - up_half) << 23);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[ks][i] = x[ks][i] * f0 * f1;
             // A 32-bit word of K codes c0 .. c3 becomes the halves c0 c1 and c2 c3; a lane's word 4 t4 .. of the first
             // 16 bytes of a k-step meets the lane's word of the second 16 bytes in one instruction each.
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                q[nh][ks][0] = pack_halves(x[ks][0] * factor, x[ks][1] * factor);
-                q[nh][ks][1] = pack_halves(x[ks][4] * factor, x[ks][5] * factor);
-                q[nh][ks][2] = pack_halves(x[ks][2] * factor, x[ks][3] * factor);
-                q[nh][ks][3] = pack_halves(x[ks][6] * factor, x[ks][7] * factor);
+                q[nh][ks][0] = pack_halves(x[ks][0], x[ks][1]);
+                q[nh][ks][1] = pack_halves(x[ks][4], x[ks][5]);
+                q[nh][ks][2] = pack_halves(x[ks][2], x[ks][3]);
+                q[nh][ks][3] = pack_halves(x[ks][6], x[ks][7]);
             }
-            row_scale[nh][0] = __shfl_sync(0xffffffffu, scale, 8 * t4);
-            row_scale[nh][1] = __shfl_sync(0xffffffffu, scale, 8 * t4 + 4);
             nan_heads |= (__shfl_sync(0xffffffffu, finite ? 0 : 1, 8 * t4) | __shfl_sync(0xffffffffu, finite ? 0 : 2, 8 * t4 + 4)) << (2 * nh);
             m[nh][0] = m[nh][1] = -INFINITY;
             l[nh][0] = l[nh][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.0f;
+        }
+        // 24, and less only where a query of 2^90 or more would bring row_scale to the end of fp32's range.
+        int down = 24;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) down = min(down, 100 + up[nh]);
+        down = max(__reduce_min_sync(0xffffffffu, down), 0);
+        k_down = down << 23;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+            const float scale = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + down - up[nh]) << 23);
+            row_scale[nh][0] = __shfl_sync(0xffffffffu, scale, 8 * t4);
+            row_scale[nh][1] = __shfl_sync(0xffffffffu, scale, 8 * t4 + 4);
         }
     }
 
@@ -228,7 +246,7 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
         const bool partial = n_valid < TILE_N || bad != 0u;
         auto valid = [&](int tok) { return tok < n_valid && ((bad >> (tok >> frag_shift)) & 1u) == 0u; };
 
-        // The scale bytes become floats once a token: K's as it is, V's relative to the unit.  Tokens that are not
+        // The scale bytes become floats once a token: K's 2^k_down too small, V's relative to the unit.  Tokens that are not
         // there get zeros, and so do their V codes: what the buffers hold for them is stale.
         uint32_t pairs = lds32<0>(sb + lane * 4);
         if (partial) {
@@ -248,9 +266,9 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
         const int old_exp = v_exp;
         v_exp = max(v_exp, top);
         const int off = (142 - v_exp) * (1 << 23);
-        sts_float4(fb + lane * 16, __uint_as_float((pairs << 23) & 0x7f800000u),
+        sts_float4(fb + lane * 16, __int_as_float(max(static_cast<int>((pairs << 23) & 0x7f800000u) - k_down, 0)),
                    __int_as_float(max(static_cast<int>((pairs << 15) & 0x7f800000u) + off, 0)),
-                   __uint_as_float((pairs << 7) & 0x7f800000u),
+                   __int_as_float(max(static_cast<int>((pairs << 7) & 0x7f800000u) - k_down, 0)),
                    __int_as_float(max(static_cast<int>((pairs >> 1) & 0x7f800000u) + off, 0)));
         __syncwarp();
         const float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);

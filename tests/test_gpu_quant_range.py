@@ -49,3 +49,52 @@ def test_a_few_large_query_elements_leave_the_small_ones_exact(dev, kind, dtype,
     plan = sa.QuantDecodePlan.build(q.to(dev), cache, kernel=kernel)
     check(plan.run(), q, mirror, [T, T - 33])
     assert plan.device_status() == 0
+
+
+def shifted(dev, code, q, k, v, query, cache_k):
+    """Query times 2^query, K rows times 2^cache_k (exactly, by their scale bytes): (device query, cache, query, mirror)."""
+    cache, mirror = written(dev, "contig", code, k, v)
+    bytes_ = mirror["scales"][..., 0].int() + cache_k
+    mirror["scales"][..., 0] = torch.where(mirror["scales"][..., 0] == 0, 0, bytes_.clamp(27, 254)).to(torch.uint8)
+    q = (q.float() * 2.0 ** query).to(q.dtype)
+    upload(cache, mirror, [k.shape[1]] * k.shape[0])
+    return q.to(dev), cache, q, mirror
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("dim,group", [(64, 5), (128, 16)])
+@pytest.mark.parametrize("power", [-112, -100, -30, 60, 94])
+def test_queries_and_keys_at_opposite_ends_of_the_range(dev, kernel, code, dim, group, power):
+    """Scores of a few units from queries of 2^power and keys of 2^-power."""
+    B, T, H = 1, 150, 2
+    k, v = (torch.randn(B, T, H, dim, generator=torch.Generator().manual_seed(s)) for s in (1, 2))
+    q = torch.randn(B, 1, H * group, dim, generator=torch.Generator().manual_seed(3)).bfloat16()
+    q[q.abs() < 2.0 ** -10] = 0.0                                          # what is left is a normal number after the shift
+    dq, cache, q, mirror = shifted(dev, code, q, k, v, power, -power)
+    check(sa.QuantDecodePlan.build(dq, cache, kernel=kernel).run(), q, mirror, [T])
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("code", list(CODES))
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 11)])
+@pytest.mark.parametrize("power", [96, 112, 118])
+def test_huge_keys_pick_their_token(dev, kernel, code, dim, group, power):
+    """Keys up to 2^119 with ordinary queries: one token's score is twice the next, so its V row is the result."""
+    B, T, H = 2, 200, 2
+    size = 1.0 - 2.0 * (torch.arange(T) % 2)                               # the others: 1 and -1
+    size[131] = 2.0
+    k = size.view(1, T, 1, 1).expand(B, T, H, dim)
+    v = torch.randn(B, T, H, dim, generator=torch.Generator().manual_seed(2))
+    q = torch.randn(B, 1, H * group, dim, generator=torch.Generator().manual_seed(3)).abs().bfloat16()
+    q[0, 0, 0] *= 2.0 ** -90                                               # next to small queries and one of zeros
+    q[0, 0, 1] = 0.0
+    dq, cache, q, mirror = shifted(dev, code, q, k, v, 0, power)
+    got = sa.QuantDecodePlan.build(dq, cache, kernel=kernel).run().cpu().double().view(B, H, group, dim)
+    value = oracle.decode(mirror["value"], mirror["scales"][..., 1])[:, :, :T]
+    want = value[:, :, 131, None].expand(B, H, group, dim).clone()
+    assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs())[:, :, 2:].all())
+    # the head of zeros weighs all tokens alike: the sum of T products in fp32, p rounded to fp16, the result to bf16
+    mean, spread = value[0, 0].mean(0), value[0, 0].abs().mean(0)
+    assert bool(((got[0, 0, 1] - mean).abs() <= 2.0 ** -8 * mean.abs() + spread * (2.0 ** -11 + T * 2.0 ** -23 + 2.0 ** -20) * 2).all())
+    assert bool(((got[0, 0, 0] - want[0, 0, 0]).abs() <= 2.0 ** -8 * want[0, 0, 0].abs()).all())
