@@ -19,9 +19,18 @@
 //
 // Every score is then multiplied by the token's K scale, 2^(e - 127 - k_down) exactly, and row_scale puts the powers
 // of two right that the query took and k_down left out.  The products are below 2^31, the codes times their scale below
-// 2^128, so scores at 2^-24 (k_down = 24) of the products stay finite for every finite K.  p is multiplied by the V scale
-// relative to a unit, 2^(e - v_exp + 15) <= 2^15 with v_exp the largest V byte so far: at the top of fp16's
-// range, where a small p or a small row of V keeps its eleven bits down to 2^-29 of the largest.
+// 2^128, so scores at 2^-24 (k_down = 24) of the products stay finite for every finite K.
+//
+// p times the V scale is rounded to fp16 (2^-11; the denominator sums p in fp32).  It is taken relative to the largest such
+// product so far, 2^(score - max + e - v_exp + lift + 15) <= 2^15 with v_exp the largest V byte so far and lift, a head's
+// own, what the row's products stay below 2^15 by: at the top of fp16's range, where a small p or a small row of V keeps
+// its eleven bits down to 2^-20 of the largest product and a part of them to 2^-30, however large the V rows are that
+// hardly count (down to 2^-100).  `room` is at least what the products stay below the bound by.  While it is below kFreeRoom,
+// as in any row whose V scales are of one order, lift is 0 and the tiles are not searched for their largest product; room
+// may then be up to kFreeRoom too large, which lift leaves out.  Beside a form that knew v_exp alone, in which 2^26 between
+// the V rows cost bits and 2^40 the smaller rows, this costs 1 % on long rows, 3 % on short ones and 4 to 6 % with 9 to 16
+// heads.  The products are made before the branch: scores that change in it, for lift to go into their exponent, hold up
+// every tile's exponentials (1M tokens, D128: 316 us without lift, 318 so, 325 that way; 16 heads, D64: 35, 37, 39).
 //
 // What bounds it: at D128 memory (8 rows x 2 KV heads x 65536 tokens, 8 heads a group: 46 us for 271 MB, 5.85 TB/s;
 // 61 x 8 x 8192 int8: 164 us, 6.3 TB/s), at D64 the instructions between two tiles as much as memory
@@ -148,6 +157,11 @@ template <int D> __device__ __forceinline__ uint32_t piece(int row, int chunk)
     return row * D + ((D == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4);
 }
 
+constexpr float kFreeRoom = 8.0f;
+
+// Powers of two by which p is raised when the products of p and V scale stay 2^room below their bound.
+__device__ __forceinline__ float lift_of(float room) { return fmaxf(floorf(fminf(room, kFreeRoom + 100.0f)) - kFreeRoom, 0.0f); }
+
 template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
     static constexpr int TILE_N = kQuantTileTokens;  // two tokens' scales a lane
     static constexpr int NH = ROWS16 ? 2 : 1;     // groups of eight heads
@@ -159,8 +173,10 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
     uint32_t q[NH][KS][4];
     int k_down;                  // (warp) powers of two left out of the K scales, as the exponent field of a float
     float row_scale[NH][2];      // heads 2 t4 and 2 t4 + 1: what turns the products into base-2 scores
-    float m[NH][2], l[NH][2];    // running maximum (in the products' unit) and this lane's part of the sum
-    float o[NH][DT][4];          // in units of 2^(v_exp - 142)
+    float m[NH][2], l[NH][2];    // running maximum (in the products' unit) and this lane's part of the sum, of 2^lift p
+    float room[NH][2];           // see above
+    bool lifted;                 // (warp) room is kFreeRoom or more for one of the heads
+    float o[NH][DT][4];          // in units of 2^(v_exp - 142 - lift)
     int v_exp;                   // largest scale byte of V so far, at least 16
     bool has_nan;                // a NaN scale was met: the result is NaN
     int nan_heads;               // bit 2 nh + h: the query of that head holds a NaN or an infinity, and its result is NaN
@@ -171,6 +187,7 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
         v_exp = 16;
         has_nan = false;
         nan_heads = 0;
+        lifted = false;
         int up[NH];  // exponent of the factor of head g of each eight, in [-113, 140]
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
@@ -221,6 +238,7 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
             nan_heads |= (__shfl_sync(0xffffffffu, finite ? 0 : 1, 8 * t4) | __shfl_sync(0xffffffffu, finite ? 0 : 2, 8 * t4 + 4)) << (2 * nh);
             m[nh][0] = m[nh][1] = -INFINITY;
             l[nh][0] = l[nh][1] = 0.0f;
+            room[nh][0] = room[nh][1] = INFINITY;
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.0f;
         }
@@ -271,7 +289,6 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
                    __int_as_float(max(static_cast<int>((pairs << 7) & 0x7f800000u) - k_down, 0)),
                    __int_as_float(max(static_cast<int>((pairs >> 1) & 0x7f800000u) + off, 0)));
         __syncwarp();
-        const float unit = __uint_as_float(static_cast<uint32_t>(max(127 + old_exp - v_exp, 0)) << 23);
 
         // Every 16-token tile has the same swizzle, so a lane's places in it are computed once a tile.
         const int row_g = tile_token<D>(g);
@@ -333,8 +350,8 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
 
         // Online softmax.  The running maximum is subtracted before row_scale is applied, so that the largest p
         // is exactly 1 however large the scores are (fma(s, scale, -max * scale) makes it 2^(rounding of the product)).
-        float sub[NH][2], alpha[NH][2];
-        bool same = unit == 1.0f;
+        float alpha[NH][2], sum[NH][2];
+        bool same = v_exp == old_exp && !lifted;
 #pragma unroll
         for (int nh = 0; nh < NH; ++nh) {
 #pragma unroll
@@ -347,19 +364,41 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 same = same && !(x > m[nh][h]);
                 x = fmaxf(m[nh][h], x);
-                sub[nh][h] = x == -INFINITY ? 0.0f : x;
-                alpha[nh][h] = m[nh][h];
+                const float sub = x == -INFINITY ? 0.0f : x;
+                alpha[nh][h] = (m[nh][h] - sub) * row_scale[nh][h];  // -inf for the first tokens
                 m[nh][h] = x;
+                // The scores become p times the V scale, before it is known whether the sums so far have to be rescaled.
+                sum[nh][h] = 0.0f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const float p0 = exp2f((s[mt][nh][h] - sub) * row_scale[nh][h]), p1 = exp2f((s[mt][nh][2 + h] - sub) * row_scale[nh][h]);
+                    sum[nh][h] += p0 + p1;
+                    s[mt][nh][h] = p0 * v_weight[mt][0];
+                    s[mt][nh][2 + h] = p1 * v_weight[mt][1];
+                }
             }
         }
-        if (!__all_sync(0xffffffffu, same)) {  // a new maximum or unit: after a row's first tiles rarely
+        if (!__all_sync(0xffffffffu, same)) {  // a new maximum or unit, or lift is in use: after a row's first tiles rarely
+            const float rise = static_cast<float>(v_exp - old_exp);
+            bool free = true;
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) free = free && room[nh][h] - alpha[nh][h] + rise < kFreeRoom;
+            if (!__all_sync(0xffffffffu, free)) {
+                lifted = find_room(s, sum, alpha, rise);
+            } else {
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) room[nh][h] = room[nh][h] - alpha[nh][h] + rise;
+            }
 #pragma unroll
             for (int nh = 0; nh < NH; ++nh) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    alpha[nh][h] = exp2f((alpha[nh][h] - sub[nh][h]) * row_scale[nh][h]);
-                    l[nh][h] *= alpha[nh][h];
-                    alpha[nh][h] *= unit;
+                    l[nh][h] *= exp2f(alpha[nh][h]);
+                    alpha[nh][h] = exp2f(alpha[nh][h] - rise);
                 }
 #pragma unroll
                 for (int i = 0; i < DT; ++i) {
@@ -371,20 +410,18 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
             }
         }
 
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+            l[nh][0] += sum[nh][0];
+            l[nh][1] += sum[nh][1];
+        }
         unrolled<MT>([&](auto mt_c) {
             constexpr int mt = decltype(mt_c)::value;
-            const float v0 = v_weight[mt][0], v1 = v_weight[mt][1];
             uint32_t b[NH][2];
 #pragma unroll
             for (int nh = 0; nh < NH; ++nh) {
-                const float p0 = exp2f((s[mt][nh][0] - sub[nh][0]) * row_scale[nh][0]);
-                const float p1 = exp2f((s[mt][nh][1] - sub[nh][1]) * row_scale[nh][1]);
-                const float p2 = exp2f((s[mt][nh][2] - sub[nh][0]) * row_scale[nh][0]);
-                const float p3 = exp2f((s[mt][nh][3] - sub[nh][1]) * row_scale[nh][1]);
-                l[nh][0] += p0 + p2;
-                l[nh][1] += p1 + p3;
-                b[nh][0] = transpose8(pack_halves(p0 * v0, p1 * v0));
-                b[nh][1] = transpose8(pack_halves(p2 * v1, p3 * v1));
+                b[nh][0] = transpose8(pack_halves(s[mt][nh][0], s[mt][nh][1]));
+                b[nh][1] = transpose8(pack_halves(s[mt][nh][2], s[mt][nh][3]));
             }
             // The lane's D/8 bytes of its four tokens; two tokens are interleaved byte by byte, so that one
             // conversion yields one operand register.  Byte 2 i is row g of output tile i, byte 2 i + 1 row g + 8.
@@ -415,6 +452,38 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
         });
     }
 
+    // Finds how far the tile's largest products w = p * (V scale) lie below their bound 2^15.  Where that leaves room they and
+    // the tile's sums of p are raised, and `fall`, by which the sums so far are scaled, takes the change of lift in.
+    // Whether one of the heads has kFreeRoom or more.
+    __device__ __forceinline__ bool find_room(float (&w)[MT][NH][4], float (&sum)[NH][2], float (&fall)[NH][2], float rise)
+    {
+        bool any = false;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float x = 0.0f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(w[mt][nh][h], w[mt][nh][2 + h]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                const float before = lift_of(room[nh][h]);
+                room[nh][h] = fminf(room[nh][h] - fall[nh][h] + rise, static_cast<float>(142 - (__float_as_int(x) >> 23)));
+                const float lift = lift_of(room[nh][h]), up = exp2f(lift);
+                sum[nh][h] *= up;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    w[mt][nh][h] *= up;
+                    w[mt][nh][2 + h] *= up;
+                }
+                fall[nh][h] += lift - before;
+                any = any || room[nh][h] >= kFreeRoom;
+            }
+        }
+        return __any_sync(0xffffffffu, any);
+    }
+
     // The warp's state into its area: rows of `stride` floats, (o[D], m, l), m in base-2 scores.
     __device__ __forceinline__ void store(float *area, int stride, int g, int t4)
     {
@@ -427,15 +496,16 @@ template <typename T, int D, bool ROWS16, int CODE> struct QuantWarp {
                 sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const float lower = lifted ? exp2f(-lift_of(room[nh][h])) : 1.0f;
                 float *row = area + (nh * 8 + 2 * t4 + h) * stride;
 #pragma unroll
                 for (int i = 0; i < DT; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        row[g * (D / 8) + 2 * i + e] = has_nan || ((nan_heads >> (2 * nh + h)) & 1) ? __uint_as_float(0x7fffffffu) : o[nh][i][2 * e + h] * unit;
+                        row[g * (D / 8) + 2 * i + e] = has_nan || ((nan_heads >> (2 * nh + h)) & 1) ? __uint_as_float(0x7fffffffu) : o[nh][i][2 * e + h] * lower * unit;
                 if (g == 0) {
                     row[D] = m[nh][h] * row_scale[nh][h];
-                    row[D + 1] = sum;
+                    row[D + 1] = sum * lower;
                 }
             }
         }
