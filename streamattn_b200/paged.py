@@ -17,6 +17,7 @@ from typing import Any, Optional
 import torch
 
 from . import native
+from .quant_cache import QuantKVCache, QuantPagedKVCache
 
 PAGED_EXACT_NATIVE_BACKEND = "streamattn_paged_exact_native"
 PAGED_EXACT_SM100_BACKEND = "streamattn_paged_sm100_exact"
@@ -164,7 +165,7 @@ class PagedExactDecodePlan:
         Triton path (``tokens_per_tile`` and friends) are accepted and ignored.
         """
 
-        if not isinstance(cache, PagedKVCache):
+        if isinstance(cache, (QuantKVCache, QuantPagedKVCache)):
             raise ValueError("cache must be a PagedKVCache (8-bit caches: QuantDecodePlan)")
         cache.validate(query, validate_metadata=validate_metadata)
         if output is None:
