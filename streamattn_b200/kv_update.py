@@ -13,6 +13,7 @@ host synchronisation and can be captured in a CUDA graph.
 
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple, Union
 
@@ -319,9 +320,12 @@ class PagedKVWriter:
         page_size = self.cache.page_size
         max_pages = int(self.cache.page_table.shape[1])
         wanted: List[Tuple[int, int, int]] = []  # (row, pages it has, pages it needs)
-        more = [tokens] * len(self.lengths) if isinstance(tokens, int) else [int(x) for x in tokens]
-        if len(more) != len(self.lengths) or min(more, default=0) < 0:
-            raise ValueError("tokens must be one number, or one per request, and not negative")
+        try:
+            more = [operator.index(tokens)] * len(self.lengths)  # also numpy's integers and tensors of one
+        except TypeError:
+            more = [operator.index(x) for x in tokens]
+            if len(more) != len(self.lengths) or min(more, default=0) < 0:
+                raise ValueError("tokens must be one number, or one per request, and not negative") from None
         for b, n in enumerate(self.lengths):
             need = -(-(n + more[b]) // page_size)
             if need > max_pages:
