@@ -439,7 +439,9 @@ SA_API int sa_paged_append_kv(const void *k_new, const void *v_new, void *k_page
  *   code  x / 2^(e - 127), exact, then rounded to the code's type (halves to even)
  * A row that holds an infinity or a NaN gets e = 255 and codes 0: it reads back as NaN and makes
  * the outputs of its KV head NaN.  The power of two makes the codes independent of the arithmetic
- * that computed them, the read-back into 16-bit types exact and a second quantisation idempotent.
+ * that computed them and the read-back exact short of the target's range.  Quantising what was read back keeps the
+ * values: int8 codes and scale bytes as well, but an e4m3 row whose largest element was rounded down to the code
+ * 224 is stored with twice the codes and the next smaller scale.
  * Scales lie head-major whatever the codes' layout is, the K and the V byte of a token side by
  * side.  No counterpart in the reference. */
 enum sa_kv_code { SA_KV_E4M3 = 1, SA_KV_INT8 = 2 };

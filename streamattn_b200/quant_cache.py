@@ -6,8 +6,9 @@ byte ``e`` (255: NaN): half the bytes of a 16-bit cache plus one per row.  ``e``
 exponent (at least 27) with ``max|x| <= top * 2 ** (e - 127)``, ``top`` being 448 for e4m3 and 127 for
 int8; a code is ``x / 2 ** (e - 127)`` rounded to the code's type, halves to even.  Dividing by a
 power of two is exact, so the codes do not depend on the arithmetic that computed them, reading back
-into bf16/fp16/fp32 is exact (short of the target's range), and quantising what was read back gives
-the same codes again.  A row that holds an infinity or a NaN is stored with ``e = 255`` and codes 0:
+into bf16/fp16/fp32 is exact (short of the target's range), and quantising what was read back keeps the
+values.  It keeps int8 codes and scale bytes too; an e4m3 row whose largest element was rounded down to the code 224
+gets twice the codes and the next smaller scale.  A row that holds an infinity or a NaN is stored with ``e = 255`` and codes 0:
 it reads back as NaN and makes the outputs of its KV head NaN.
 
 Scales lie head-major whatever the codes' layout is, the K and the V byte of a token side by side:
