@@ -56,8 +56,10 @@ def _optional_counts(t: Optional[torch.Tensor], batch: int, name: str) -> int:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two contiguous tensors share memory."""
+    """Whether two contiguous tensors share memory.  Of others (slices of one buffer may interleave) only their start is compared."""
 
+    if not (a.is_contiguous() and b.is_contiguous()):
+        return a.data_ptr() == b.data_ptr()
     return a.device == b.device and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() \
         and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
 
@@ -128,7 +130,7 @@ class QuantizeKVPlan(AppendKVPlan):
             raise ValueError("positions must have the dtype of the lengths that are written")
         pos_dtype, num_positions = _positions(positions, batch, lengths_out)
         counts_dtype = _optional_counts(counts, batch, "counts")
-        if any(_folded(t) for t in (cache.key, cache.value, cache.scales)) or cache.key.data_ptr() == cache.value.data_ptr():
+        if any(_folded(t) for t in (cache.key, cache.value, cache.scales)) or _overlap(cache.key, cache.value):
             raise ValueError("the rows of a cache that is written must not share memory")
         if lengths_out is not None and counts is not None and _overlap(lengths_out, counts):
             raise ValueError("counts must not alias the lengths that are written")
@@ -146,8 +148,10 @@ class QuantizeKVPlan(AppendKVPlan):
             if out_shape != shape or (shape[0], shape[1], shape[3]) != (batch, tokens, dim) \
                     or query.dtype != dtype or query_out.dtype != dtype:
                 raise ValueError("query / query_out must match the new rows in batch, tokens, head_dim and dtype")
-            if query_out.data_ptr() == query.data_ptr():
+            if _overlap(query_out, query):
                 raise ValueError("query_out must not alias query")
+            if any(_overlap(query_out, t) for t in (key_new, value_new)):
+                raise ValueError("query_out must not alias the new rows")
             if _folded(query_out):
                 raise ValueError("the rows of query_out must not share memory")
             q_heads = shape[2]
@@ -231,7 +235,7 @@ class DequantizeKVPlan:
         counts_dtype = _optional_counts(counts, batch, "counts")
         if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
             raise ValueError("status must be an int32 tensor")
-        if _folded(key_out) or key_out.data_ptr() == value_out.data_ptr():
+        if _folded(key_out) or _overlap(key_out, value_out):
             raise ValueError("the rows of key_out and value_out must not share memory")
         device = native.require_cuda(*cache.tensors(), key_out, value_out, starts, counts, status)
         desc = cache.descriptor()

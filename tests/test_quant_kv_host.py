@@ -300,3 +300,27 @@ def test_oracle_scales_and_codes():
         assert bool(((oracle.decode(c, e) - y).abs() <= bound).all())
         again, e2 = oracle.encode(oracle.decode(c, e), code)
         assert torch.equal(oracle.decode(again, e2), oracle.decode(c, e))
+
+
+def test_partly_overlapping_operands_are_refused():
+    """Contiguous operands that share a part of their memory; slices of one buffer that interleave are fine."""
+    buffer = torch.zeros(5, 3, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="must not alias query"):
+        sa.quantize_kv(contig(), K, K, query=buffer[:2], query_out=buffer[1:3])
+    with pytest.raises(ValueError, match="must not alias the new rows"):
+        sa.quantize_kv(contig(), buffer[:2], K, query=K, query_out=buffer[1:3])
+    with pytest.raises(ValueError, match="must not alias the new rows"):
+        sa.quantize_kv(contig(), K, K, query=buffer[:2], query_out=K)
+    with pytest.raises(ValueError, match="value_out must not share memory"):
+        sa.DequantizeKVPlan.build(contig(), buffer[:2], buffer[1:3])
+    codes = torch.zeros(3, 4, 16, 64, dtype=torch.int8)
+    with pytest.raises(ValueError, match="must not share memory"):
+        sa.quantize_kv(contig(key=codes[:2], value=codes[1:]), K, K)
+    fused = torch.zeros(2, 3, 16, 64, dtype=torch.bfloat16)                # heads of K, V, the query and its result side by side
+    k, v, q, out = fused.split(4, dim=2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        sa.quantize_kv(contig(), k, v, query=q, query_out=out)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        sa.DequantizeKVPlan.build(contig(), k, v)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        sa.quantize_kv(contig(), buffer[:2], buffer[2:4], query=K, query_out=torch.empty_like(K))
