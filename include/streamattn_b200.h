@@ -510,6 +510,10 @@ SA_API int sa_dequantize_kv(const sa_quant_cache_t *cache, void *k_out, void *v_
  * sa_paged_decode (paged cache; seq_lens required, trace optional).  The plan form is run with
  * sa_plan_run and takes sa_plan_set_rows and sa_plan_set_wait_limit_ns.  Tokens of a bad page are
  * left out of the softmax and reported (SA_DEV_BAD_PAGE).
+ * Arithmetic: the query is used as it is (the streaming kernel rounds an element that is 2^28 times smaller than the
+ * largest of its head, subnormal ones count as zeros), scores, probabilities and sums are fp32, and the streaming kernel
+ * rounds a probability times its token's V scale to fp16: 2^-11 of it at most, or 2^-31 of the largest such product of the
+ * head where that is more.  Finite queries and caches give finite results as long as the scores and sums fit fp32.
  */
 SA_API int sa_quant_decode(const void *q, const sa_quant_cache_t *cache, void *out,
                            void *workspace, size_t workspace_bytes, const void *seq_lens, int lens_dtype,

@@ -245,9 +245,9 @@ bool build_stream_geometry(const Problem &p, int64_t max_vlen, StreamGeometry *g
         if (quant) {
             // 8-bit caches: n CTAs for each (row, KV head) pair stream its t tiles in a time that falls with t / n and merge
             // their states in one that grows with n, which is least near n = 1.25 sqrt(t) (one pair, 8 heads, D64: 16384
-            // tokens 8.5 us with 20 CTAs, 13.3 with 64; 131072 tokens 18.0 with 48 to 64, 22.8 with 148).  At least one CTA
-            // each: a CTA's pairs are finished one after the other (16 pairs of one tile, 16 heads each: 16.7 us with 4
-            // CTAs, 5.4 with 16).
+            // tokens 10.4 us with 20 CTAs, 12.4 with 8, 15.2 with 64; 131072 tokens 19.4 with 57, 25.3 with 20, 25.9 with 148;
+            // 4 pairs of 4096 8.3 with 40, 9.8 with 16, 8.9 with 64).  At least one CTA each: a CTA's pairs are finished
+            // one after the other (16 pairs of one tile, 16 heads each: 19.7 us with 4 CTAs, 7.2 with 16).
             const int64_t pairs = static_cast<int64_t>(p.batch) * p.kv_heads * geo->kv_split;
             ctas = pairs * static_cast<int64_t>(std::ceil(1.25 * std::sqrt(static_cast<double>(tiles / pairs))));
         }

@@ -9,12 +9,14 @@
 // such accesses (D no multiple of 16, odd strides) take one warp a unit with single-element accesses.
 //
 // Measured (bytes as above against the time): 8 x 4096 tokens x 2 heads, D64, bf16 with rotation and 16 query heads to
-// e4m3 32.1 us, 5.2 TB/s; 13 ragged rows of up to 8190 tokens x 8 heads, D128, fp16 to int8 in token-major pages 88 us,
-// 4.9 TB/s; read back: ragged 8 x 65536 x 2, D64, pages of 16 46 us, 5.9 TB/s; 3 x 32768 x 8, D128, int8 to fp16 91 us,
-// 6.6 TB/s.  One token a row (8 rows, 2 + 16 heads): 6.0 us, the launch and one chain of position, page id and rows.
+// e4m3 31.0 us, 5.4 TB/s; 13 ragged rows of up to 8190 tokens x 8 heads, D128, fp16 to int8 in token-major pages 80 to 82 us,
+// 5.3 TB/s; read back: ragged 8 x 65536 x 2, D64, pages of 16 46 to 50 us (the lengths are drawn), 5.4 to 5.9 TB/s;
+// 3 x 32768 x 8, D128, int8 to fp16 91.6 us, 6.6 TB/s.  One token a row (8 rows, 2 + 16 heads): 6.0 us, the launch and one
+// chain of position, page id and rows.  8 x 4096 x 2 heads without rotation: D48 7.4 us written and 5.2 read in pieces,
+// D40 29.8 and 13.1 by single elements, which nothing but being right was asked of.
 // What made the difference: pieces of both halves of a row in one lane, so that rotation needs no other lane and each
-// unit costs half the index arithmetic (write 190 -> 91 us, 66 -> 33; read 113 -> 91, 59 -> 44).  Putting the
-// page id's look-up behind the row loads gained nothing.
+// unit costs half the index arithmetic; it halved the writes.  Putting the page id's look-up behind the row loads gained
+// nothing.
 #include <algorithm>
 
 #include "sa_quant.cuh"
@@ -208,8 +210,8 @@ template <typename T> struct Halves {
     }
 };
 
-// 16-bit rows: registers for five CTAs an SM with rotation (48; 64 and four without the bound: 33.2 -> 32.1 us for the chunk
-// above), for six without (40; five: 91.2 -> 88.8 us for the prompts).
+// 16-bit rows: registers for five CTAs an SM with rotation (48; 64 and four without the bound, which takes 3 % more for
+// the chunk above), for six without (40; five take 3 % more for the prompts).
 template <typename T, int CODE, bool ROPE>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? (ROPE ? 5 : 6) : 1) quantize_vector_kernel(const __grid_constant__ QuantizeParams p, int lane_shift)
 {

@@ -15,9 +15,8 @@ constexpr int kStreamWarps = SA_STREAM_WARPS;    // each with its own ring of ti
 constexpr int kStreamStages = SA_STREAM_STAGES;  // 16 KB K+V tiles in flight per warp
 
 // 8-bit caches: tiles of 64 tokens, 8 KB of codes at D64 and 16 KB at D128, and 16 KB in flight a warp at either.
-// Tried at 8 rows x 2 KV heads x 65536 tokens, D64 (24.9 us, 27.5 in pages of 64): tiles of 128 tokens leave a
-// coarser last round; a third stage, or 10, 12 or 16 warps, spill or keep fewer bytes in flight - 12 warps gain 1-2 us in
-// pages and lose 2.7 on rows.
+// Tried at 8 rows x 2 KV heads x 65536 tokens, D64: tiles of 128 tokens leave a coarser last round; a third stage, or 10, 12
+// or 16 warps, spill or keep fewer bytes in flight - 12 warps gain 1-2 us in pages and lose 2.7 on rows.
 constexpr int kQuantTileTokens = 64;
 
 // Tiles in flight per warp.

@@ -613,9 +613,9 @@ struct Frag {
 
 // SOLO (8-bit caches, more pairs than CTAs, so that every slice crosses pairs): each warp streams a part of the CTA's slice
 // by itself, without a barrier between pairs.  A pair that lies in one warp's part is finished by that warp; the others, one for
-// each border between parts at most, are combined by the whole CTA afterwards.  With a barrier a pair instead: 1024 pairs of 128
-// to 1024 tokens, D128, 94 us against 54; 256 of 128 to 2048 43 and 28; 488 of 512 to 2048, D64, 52 and 35; 488 of 2048 to 8192,
-// int8, D128, 121 and 111.  With fewer pairs the cut by warps gains nothing, and choosing at run time costs 1 us.
+// each border between parts at most, are combined by the whole CTA afterwards.  With a barrier a pair instead (pages
+// of 64): 1024 pairs of 128 to 1024 tokens, D128, 96 us against 53.5; 256 of 128 to 2048 48 and 32; 488 of 512 to 2048, D64,
+// 53 and 36; 488 of 2048 to 8192, int8, D128, 141 and 130.  An instance of its own, so that the others keep their loop.
 template <typename T, int D, int WARPS, int STAGES, bool ROWS16, int CODE, int PLACE, bool SOLO>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -752,10 +752,8 @@ stream_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     // that many each, whole CTAs to a pair, ceil(tiles / level) of them.  Equal slices would give total / C each, but a slice
     // that crosses pairs costs its CTA a second segment, some 3 us, and with many pairs every CTA has one or two and most
     // pairs are merged; so the CTAs are aligned while level is at most 2 + 8 pairs / C rounds of the warps above that (aligned and
-    // not: 128 pairs of 2048 tokens, D128, 14.2 and 18.7 us; 120 of 4096, D64, 16.6 and 19.0; 120 of 1024 to 8192, 25.5 and
-    // 29.6; 144 of 100 to 8192, 32 and 40; 48 of 30000 to 65536, D128, 105 and 99; 16 of 524288 170 and 166).
-    // Levels against slices rounded to pairs one after the other: 24 pairs of 16384 to 65536 29.5 -> 27.4 us, 32 of 8192 to
-    // 32768, int8, 25.5 -> 22.8.
+    // not: 128 pairs of 2048 tokens, D128, 17.6 and 22.6 us; 120 of 4096, D64, 17.6 and 21.2; 120 of 1024 to 8192, 26.4 and
+    // 31.2; 144 of 100 to 8192, 28.2 and 38.2; 48 of 30000 to 65536, D128, and 16 of 524288, D64, the same, 97.5 and 175).
     auto align_quant = [&]() {
         aligned = false;
         if (total_tiles > 0 && num_pairs <= C) {

@@ -30,16 +30,18 @@
 // may then be up to kFreeRoom too large, which lift leaves out.  Beside a form that knew v_exp alone, in which 2^26 between
 // the V rows cost bits and 2^40 the smaller rows, this costs 1 % on long rows, 3 % on short ones and 4 to 6 % with 9 to 16
 // heads.  The products are made before the branch: scores that change in it, for lift to go into their exponent, hold up
-// every tile's exponentials (1M tokens, D128: 316 us without lift, 318 so, 325 that way; 16 heads, D64: 35, 37, 39).
+// every tile's exponentials, another 2 to 6 %.
 //
-// What bounds it: at D128 memory (8 rows x 2 KV heads x 65536 tokens, 8 heads a group: 46 us for 271 MB, 5.85 TB/s;
-// 61 x 8 x 8192 int8: 164 us, 6.3 TB/s), at D64 the instructions between two tiles as much as memory
-// (24.9 us, 5.48 TB/s, of which 5 us are launch, first tile and merge).  Groups of 9 to 16 heads do the second
-// product twice per conversion and are bound by issue: 32 us at D64.  int8 costs 2.5 us more than e4m3 there: a byte
-// pair becomes two halves in five instructions against one.  What made the difference, at that D64 shape:
-// heads on M, tokens on N and one tile in four used 36.7 us; tokens on M (no padded rows) 33; e4m3 as fp16 instead
-// of e4m3 instructions 29.4; scales as floats once a token, places once a tile, the rescale skipped while the
-// maximum stands 27.2; instances by where the tokens lie 24.9.
+// What bounds it (8 rows x 2 KV heads x 65536 tokens unless said otherwise): at D64 the instructions between two tiles as much
+// as memory: 27.0 us, 5.05 TB/s, of which 5 us are launch, first tile and merge; 29.4 in pages of 64, 33.4 of 16.  Groups of
+// 9 to 16 heads do both products twice per conversion and are bound by issue: 35.2 us.  int8 takes 30.8 and 38.6 us there: a
+// word of codes becomes halves in five instructions against two.  At D128 a warp has one tile in flight, so what it
+// computes adds to the wait for the next: 50.3 us e4m3, 5.4 TB/s, 55 int8, and 62 and 69 with 16 heads; with 8 KV heads of 4 and
+// 1M tokens 336 and 347 us, 6.4 and 6.2 TB/s (int8 by integer products, which lost small elements of the query: 325).  What
+// made the difference at first, at that D64 shape (its codes drawn uniformly): heads on M, tokens on N and one tile in four
+// used 36.7 us; tokens on M (no padded rows) 33; e4m3 as fp16 instead of e4m3 instructions 29.4; scales as floats
+// once a token, places once a tile, the rescale skipped while the maximum stands 27.2; instances by where the tokens
+// lie 24.9.
 #pragma once
 
 #include <type_traits>

@@ -104,8 +104,6 @@ _SIGNATURES = {
     "sa_set_wait_limit_ns": ([ctypes.c_uint64], _i),
     "sa_plan_set_wait_limit_ns": ([_vp, ctypes.c_uint64], _i),
     "sa_o_proj": ([_vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i, _i, _vp], _i),
-    # k_new v_new k_cache v_cache | positions pos_dtype num_positions lens_out | cos sin rope_stride_b |
-    # q_in q_out q_heads 4 q strides | batch kv_heads head_dim kv_len | 2 new strides | 3 kv strides | dtype status stream
     "sa_quant_decode": (_QUANT_ARGS + [_vp], _i),
     "sa_quant_plan_create": (_QUANT_ARGS, _vp),
     # cache | k_new v_new tokens 3 strides | positions pos_dtype num_positions | counts counts_dtype | lens_out |
@@ -115,6 +113,8 @@ _SIGNATURES = {
     # cache | k_out v_out tokens 3 strides | starts dtype | counts dtype | dtype status stream
     "sa_dequantize_kv": ([ctypes.POINTER(QuantCacheStruct), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i, _vp, _i, _i,
                           _vp, _vp], _i),
+    # k_new v_new k_cache v_cache | positions pos_dtype num_positions lens_out | cos sin rope_stride_b |
+    # q_in q_out q_heads 4 q strides | batch kv_heads head_dim kv_len | 2 new strides | 3 kv strides | dtype status stream
     "sa_append_kv": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _i64,
                       _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i, _vp, _vp], _i),
     # ... k_pages v_pages page_table table_dtype | positions ... | batch kv_heads head_dim page_size max_pages

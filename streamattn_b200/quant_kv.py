@@ -295,6 +295,10 @@ class QuantDecodePlan:
         ``[B, Hq, D + 2]`` (what ``sa_merge_states`` joins).  ``splits``, ``kernel``, ``record_page_walk`` (paged caches) and ``row_indices`` as in :class:`PagedExactDecodePlan` and
         :class:`ExactDecodePlan`; ``validate_metadata`` checks a paged cache's lengths and page ids
         on the host, once.  Rows of no tokens give zeros.
+
+        Scores, probabilities and sums are fp32 on both kernels and the query is used as it is; the
+        tensor-core kernel rounds a probability times its token's V scale to fp16 before it meets the
+        codes (2^-11 of the product, or 2^-31 of the head's largest).
         """
 
         _cache(cache)
