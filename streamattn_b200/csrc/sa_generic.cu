@@ -5,6 +5,8 @@
 // a scale byte a row, see sa_quant.cuh).  One CTA handles one (row, query head, split); a
 // second launch merges the split states exactly.  Also hosts the state-merge
 // kernel used after the cross-GPU gather of context-parallel decode.
+#include <algorithm>
+
 #include "sa_quant.cuh"
 
 namespace sa {
@@ -71,7 +73,8 @@ generic_partial_kernel(const __grid_constant__ GenericParams p)
     __shared__ float sm_l[kGenericWarps];
     __shared__ float sm_o[kGenericWarps][kMaxDim];
 
-    const int pair = blockIdx.y;
+    const int pair = blockIdx.z * gridDim.y + blockIdx.y;
+    if (pair >= p.batch * p.q_heads) return;
     const int split = blockIdx.x;
     const int b = pair / p.q_heads;
     const int h = pair % p.q_heads;
@@ -289,7 +292,9 @@ cudaError_t launch_generic_typed(const Problem &p, int splits, cudaStream_t stre
     gp.scale_log2 = kLog2e / sqrtf(static_cast<float>(p.head_dim));
     gp.quant = p.quant;
     const int pairs = p.batch * p.q_heads;
-    dim3 grid(splits, pairs);
+    // The second dimension of a grid ends at 65535: more (row, query head) pairs go on in the third.
+    constexpr int kMaxGridY = 65535;
+    dim3 grid(splits, std::min(pairs, kMaxGridY), (pairs + kMaxGridY - 1) / kMaxGridY);
     generic_partial_kernel<T, CODE><<<grid, kGenericThreads, 0, stream>>>(gp);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess || splits == 1) return err;
