@@ -6,7 +6,7 @@
 //   O^T[dim, head]  += V^T P^T
 //
 // q is multiplied by the power of two that brings its largest element to [2^14, 2^15) and becomes fp16: exact for
-// all but elements some 2^30 times smaller than that one.  The codes of K and of V are converted to fp16, in which
+// all but elements some 2^28 times smaller than that one.  The codes of K and of V are converted to fp16, in which
 // either type of them is exact, and the products accumulate in fp32.
 // e4m3   There is an instruction with e4m3 operands, but on this GPU it executes as conversions and fp16 products:
 //        measured 10 instructions and 16 cycles of the tensor pipe for its 16 x 8 x 32, where two fp16
@@ -33,8 +33,8 @@
 // every tile's exponentials, another 2 to 6 %.
 //
 // What bounds it (8 rows x 2 KV heads x 65536 tokens unless said otherwise): at D64 the instructions between two tiles as much
-// as memory: 27.0 us, 5.05 TB/s, of which 5 us are launch, first tile and merge; 29.4 in pages of 64, 33.4 of 16.  Groups of
-// 9 to 16 heads do both products twice per conversion and are bound by issue: 35.2 us.  int8 takes 30.8 and 38.6 us there: a
+// as memory: 27.0 to 27.9 us (boxes differ), 4.9 to 5.05 TB/s, of which 5 us are launch, first tile and merge; 29.4 in pages of
+// 64, 33.4 of 16.  Groups of 9 to 16 heads do both products twice per conversion and are bound by issue: 35.2 us.  int8 takes 30.8 and 38.6 us there: a
 // word of codes becomes halves in five instructions against two.  At D128 a warp has one tile in flight, so what it
 // computes adds to the wait for the next: 50.3 us e4m3, 5.4 TB/s, 55 int8, and 62 and 69 with 16 heads; with 8 KV heads of 4 and
 // 1M tokens 336 and 347 us, 6.4 and 6.2 TB/s (int8 by integer products, which lost small elements of the query: 325).  What
